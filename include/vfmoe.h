@@ -212,11 +212,39 @@ int vfmoe_forward_rows(int64_t handle, int64_t rows, int64_t rows_dtype, int64_t
                        int64_t workspace, int64_t ws_bytes, int64_t stream);
 
 /* Weighted combine: out[t] = sum_l w[t,l] * y[pos_of[t*k+l]] + y_shared[t].  y rows and
- * y_shared are y_dtype VFMOE_DT_F32 or VFMOE_DT_F16; w may be 0 for weight 1; y_shared may
- * be 0; a negative pos_of entry skips that lane.  out_dtype F32, BF16 or F16.
- * glm_engine.vyb:2925-2938, :2991. */
+ * y_shared are y_dtype F32, F16 or BF16; w may be 0 for weight 1; y_shared may
+ * be 0; a negative pos_of entry skips that lane (its weight is not read into the sum).  out_dtype
+ * F32, BF16 or F16.  Any H; H a multiple of 16 bytes of y and 16-byte aligned pointers move 16-byte
+ * words.  Lanes are added in lane order in fp32, one rounding.  glm_engine.vyb:2925-2938, :2991. */
 int vfmoe_combine(int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w, int64_t T, int64_t k, int64_t H,
                   int64_t y_shared, int64_t out, int64_t out_dtype, int64_t stream);
+
+/* Gradient of vfmoe_combine with respect to the expert rows and the weights, from dout [T, H]
+ * (dout_dtype): for every lane with pos = pos_of[t*k+l] >= 0
+ *   dy[pos] = w[t,l] * dout[t]        (y_dtype, one rounding; rows that no lane names stay as they were)
+ *   dw[t,l] = <dout[t], y[pos]>       (fp32; 0 for a lane without a row)
+ * dy or dw may be 0 (y is read for dw only); w = 0: weight 1; dy may be y itself.  The gradient of
+ * y_shared is dout.  No counterpart in the reference, whose MoE path is forward only. */
+int vfmoe_combine_backward(int64_t dout, int64_t dout_dtype, int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w,
+                           int64_t T, int64_t k, int64_t H, int64_t dy, int64_t dw, int64_t stream);
+
+/* Tokens sorted by expert, in their own type: the canonical permutation of vfmoe_dispatch and a copy of
+ * every token's row x [T, H] (dtype F32, F16 or BF16) at each of its positions in xs [T*k, H].
+ * An id outside [0, n_experts) is a dropped lane (padding, capacity): it has no row, which is no
+ * error here.  A token may name one expert on several lanes; rows are ordered by (expert, token, lane).
+ *   counts [n_experts], offsets [n_experts + 1], perm_tok [T*k], pos_of [T*k]: as vfmoe_dispatch;
+ *   perm_tok is -1 from row offsets[n_experts] on, and those rows of xs stay as they were.
+ * x = 0 makes the plan alone.  n_experts <= 1024, k <= 32, T*k <= 2^30.  workspace: at least
+ * vfmoe_permute_workspace_bytes (0 for decode batches); calls that overlap on the GPU need one each. */
+int64_t vfmoe_permute_workspace_bytes(int64_t T, int64_t k, int64_t n_experts);
+int vfmoe_permute(int64_t idx, int64_t T, int64_t k, int64_t n_experts, int64_t x, int64_t dtype, int64_t H,
+                  int64_t xs, int64_t counts, int64_t offsets, int64_t perm_tok, int64_t pos_of, int64_t workspace,
+                  int64_t ws_bytes, int64_t stream);
+
+/* Gradient of the sorted rows: dx[t] = sum over the token's lanes with a row of dxs[pos_of[t*k+l]], in
+ * lane order in fp32, rounded once to dx_dtype (a token without rows gets zeros). */
+int vfmoe_permute_backward(int64_t dxs, int64_t dtype, int64_t pos_of, int64_t T, int64_t k, int64_t H, int64_t dx,
+                           int64_t dx_dtype, int64_t stream);
 
 /* Bytes of workspace vfmoe_forward_routed needs for up to n_max rows of k lanes. */
 int64_t vfmoe_routed_workspace_bytes(int64_t handle, int64_t n_max, int64_t k);

@@ -721,18 +721,90 @@ int vfmoe_forward_routed(int64_t handle, int64_t rows, int64_t rows_dtype, int64
                      reinterpret_cast<cudaStream_t>(stream));
 }
 
+static bool is_float_dtype(int64_t d) { return d == VFMOE_DT_F32 || d == VFMOE_DT_F16 || d == VFMOE_DT_BF16; }
+static int64_t dtype_bytes(int64_t d) { return d == VFMOE_DT_F32 ? 4 : 2; }
+// bounds shared by the calls on (token, lane) rows
+static bool lanes_ok(int64_t T, int64_t k, int64_t H) {
+    return T >= 0 && k > 0 && k <= 32 && T <= ((int64_t)1 << 30) / k && H > 0 && H <= ((int64_t)1 << 30);
+}
+
 int vfmoe_combine(int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w, int64_t T, int64_t k, int64_t H,
                   int64_t y_shared, int64_t out, int64_t out_dtype, int64_t stream) {
-    if (T < 0 || k <= 0 || k > 32 || H <= 0 || H % 4 || (y_dtype != VFMOE_DT_F32 && y_dtype != VFMOE_DT_F16) ||
-        (out_dtype != VFMOE_DT_F32 && out_dtype != VFMOE_DT_BF16 && out_dtype != VFMOE_DT_F16) ||
-        (T > 0 && (!y || !pos_of || !out)) || (y & 15) || (y_shared & 15)) {
+    if (!lanes_ok(T, k, H) || !is_float_dtype(y_dtype) || !is_float_dtype(out_dtype) ||
+        (T > 0 && (!y || !pos_of || !out)) || (y | y_shared) % dtype_bytes(y_dtype) || out % dtype_bytes(out_dtype) ||
+        (pos_of | w) % 4) {
         set_error("vfmoe_combine: bad arguments");
         return VFMOE_ERR_INVALID;
     }
-    return launch_combine(reinterpret_cast<const void *>(y), (int)y_dtype, reinterpret_cast<const int32_t *>(pos_of),
-                          reinterpret_cast<const float *>(w), (int)T, (int)H, (int)k,
-                          reinterpret_cast<const void *>(y_shared), reinterpret_cast<void *>(out), (int)out_dtype,
-                          reinterpret_cast<cudaStream_t>(stream));
+    if (T == 0) return VFMOE_OK;
+    return launch_return_rows(reinterpret_cast<const void *>(y), (int)y_dtype, reinterpret_cast<const int32_t *>(pos_of),
+                              reinterpret_cast<const float *>(w), T, H, (int)k, reinterpret_cast<const void *>(y_shared),
+                              reinterpret_cast<void *>(out), (int)out_dtype, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int vfmoe_combine_backward(int64_t dout, int64_t dout_dtype, int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w,
+                           int64_t T, int64_t k, int64_t H, int64_t dy, int64_t dw, int64_t stream) {
+    if (!lanes_ok(T, k, H) || !is_float_dtype(y_dtype) || !is_float_dtype(dout_dtype) ||
+        (T > 0 && (!dout || !pos_of || (!dy && !dw) || (dw && !y))) || (y | dy) % dtype_bytes(y_dtype) ||
+        dout % dtype_bytes(dout_dtype) || (pos_of | w | dw) % 4) {
+        set_error("vfmoe_combine_backward: bad arguments");
+        return VFMOE_ERR_INVALID;
+    }
+    if (T == 0) return VFMOE_OK;
+    return launch_combine_backward(reinterpret_cast<const void *>(dout), (int)dout_dtype,
+                                   reinterpret_cast<const void *>(y), (int)y_dtype,
+                                   reinterpret_cast<const int32_t *>(pos_of), reinterpret_cast<const float *>(w), T, H,
+                                   (int)k, reinterpret_cast<void *>(dy), reinterpret_cast<float *>(dw),
+                                   reinterpret_cast<cudaStream_t>(stream));
+}
+
+int64_t vfmoe_permute_workspace_bytes(int64_t T, int64_t k, int64_t n_experts) {
+    if (!lanes_ok(T, k, 1) || n_experts <= 0 || n_experts > 1024) {
+        set_error("vfmoe_permute_workspace_bytes: bad arguments");
+        return VFMOE_ERR_INVALID;
+    }
+    return permute_ws_bytes(T, (int)k, (int)n_experts);
+}
+
+int vfmoe_permute(int64_t idx, int64_t T, int64_t k, int64_t n_experts, int64_t x, int64_t dtype, int64_t H,
+                  int64_t xs, int64_t counts, int64_t offsets, int64_t perm_tok, int64_t pos_of, int64_t workspace,
+                  int64_t ws_bytes, int64_t stream) {
+    if (!lanes_ok(T, k, x ? H : 1) || n_experts <= 0 || n_experts > 1024 || !counts || !offsets ||
+        (T > 0 && (!idx || !perm_tok || !pos_of)) || (idx | counts | offsets | perm_tok | pos_of | workspace) % 4 ||
+        (x && (!is_float_dtype(dtype) || !xs || (x | xs) % dtype_bytes(dtype)))) {
+        set_error("vfmoe_permute: bad arguments");
+        return VFMOE_ERR_INVALID;
+    }
+    const int64_t need = permute_ws_bytes(T, (int)k, (int)n_experts);
+    if (need && (!workspace || ws_bytes < need)) {
+        set_error("vfmoe_permute: workspace of %lld bytes, %lld needed", (long long)(workspace ? ws_bytes : 0),
+                  (long long)need);
+        return VFMOE_ERR_WORKSPACE;
+    }
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    if (T == 0) {
+        VF_CUDA(cudaMemsetAsync(reinterpret_cast<void *>(counts), 0, n_experts * sizeof(int32_t), st));
+        VF_CUDA(cudaMemsetAsync(reinterpret_cast<void *>(offsets), 0, (n_experts + 1) * sizeof(int32_t), st));
+        return VFMOE_OK;
+    }
+    return launch_permute(reinterpret_cast<const int32_t *>(idx), T, (int)k, (int)n_experts,
+                          reinterpret_cast<const void *>(x), (int)dtype, H, reinterpret_cast<void *>(xs),
+                          reinterpret_cast<int32_t *>(counts), reinterpret_cast<int32_t *>(offsets),
+                          reinterpret_cast<int32_t *>(perm_tok), reinterpret_cast<int32_t *>(pos_of),
+                          reinterpret_cast<int32_t *>(workspace), st);
+}
+
+int vfmoe_permute_backward(int64_t dxs, int64_t dtype, int64_t pos_of, int64_t T, int64_t k, int64_t H, int64_t dx,
+                           int64_t dx_dtype, int64_t stream) {
+    if (!lanes_ok(T, k, H) || !is_float_dtype(dtype) || !is_float_dtype(dx_dtype) ||
+        (T > 0 && (!dxs || !pos_of || !dx)) || dxs % dtype_bytes(dtype) || dx % dtype_bytes(dx_dtype) || pos_of % 4) {
+        set_error("vfmoe_permute_backward: bad arguments");
+        return VFMOE_ERR_INVALID;
+    }
+    if (T == 0) return VFMOE_OK;
+    return launch_return_rows(reinterpret_cast<const void *>(dxs), (int)dtype,
+                              reinterpret_cast<const int32_t *>(pos_of), nullptr, T, H, (int)k, nullptr,
+                              reinterpret_cast<void *>(dx), (int)dx_dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int vfmoe_dispatch(int64_t idx, int64_t T, int64_t k, int64_t n_experts, int64_t counts, int64_t offsets,

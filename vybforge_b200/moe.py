@@ -16,11 +16,12 @@ kernel reached through the C ABI.  A missing library raises on import.
 from __future__ import annotations
 
 import ctypes as C
+from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from ._lib import check, DT_BF16, DT_F16, DT_F32, WFMT_Q8_0, WFMT_EXL3, WFMT_Q8_0_TILED
+from ._lib import check, VfmoeError, ERR_INVALID, DT_BF16, DT_F16, DT_F32, WFMT_Q8_0, WFMT_EXL3, WFMT_Q8_0_TILED
 from ._lib import PATH_AUTO, PATH_SIMT, PATH_TC, PATH_GEMV, PATH_TC1
 
 _PATHS = {"auto": PATH_AUTO, "simt": PATH_SIMT, "tc": PATH_TC, "gemv": PATH_GEMV, "tc1": PATH_TC1}
@@ -269,16 +270,110 @@ def dispatch(idx: torch.Tensor, n_experts: int, err: torch.Tensor | None = None)
     return perm, pos, offsets[:n_experts + 1], counts[:n_experts]
 
 
+def _need(ok: bool, msg: str) -> None:
+    if not ok:
+        raise VfmoeError(ERR_INVALID, msg)
+
+
+def _check(t: torch.Tensor, name: str, dtypes, shape) -> None:
+    """t is a contiguous tensor of one of `dtypes` on the current device with `shape` (-1: any size)."""
+    if (t.dtype not in dtypes or t.dim() != len(shape) or not t.is_contiguous() or not t.is_cuda
+            or t.device.index != torch.cuda.current_device()
+            or any(want >= 0 and have != want for have, want in zip(t.shape, shape))):
+        raise VfmoeError(ERR_INVALID, f"{name}: a contiguous tensor {list(shape)} of {[str(d) for d in dtypes]} on the "
+                                      f"current CUDA device is needed, got {list(t.shape)} {t.dtype} on {t.device}"
+                                      f"{'' if t.is_contiguous() else ', not contiguous'}")
+
+
+_I32, _F32, _FLOATS = (torch.int32,), (torch.float32,), (torch.float32, torch.float16, torch.bfloat16)
+
+
+class Plan(NamedTuple):
+    """Rows sorted by expert: row perm position i holds token perm_tok[i] (-1 behind the last row); lane (t, l)
+    has row pos_of[t*k + l] (-1: dropped); expert e's rows are [offsets[e], offsets[e + 1])."""
+    perm_tok: torch.Tensor
+    pos_of: torch.Tensor
+    offsets: torch.Tensor
+    counts: torch.Tensor
+
+
+def permute(x: torch.Tensor | None, idx: torch.Tensor, n_experts: int, out: torch.Tensor | None = None):
+    """(xs, Plan): the rows of x [T, H] sorted by the expert ids idx int32 [T, k], xs [T*k, H] of x's dtype
+    (vfmoe_permute).  An id outside [0, n_experts) drops its lane; the rows of xs behind offsets[-1] stay as
+    they were (undefined when `out` is not given).  x=None makes the plan alone (xs None)."""
+    _check(idx, "idx", _I32, (-1, -1))
+    T, k = idx.shape
+    H, dt, xs = 0, DT_F32, None
+    if x is not None:
+        _check(x, "x", _FLOATS, (T, -1))
+        H, dt = x.shape[1], _DT[x.dtype]
+        if out is None:
+            xs = torch.empty((T * k, H), dtype=x.dtype, device=x.device)
+        else:
+            _check(out, "out", (x.dtype,), (T * k, H))
+            xs = out
+    lib = _lib.load()
+    ws_bytes = check(lib.vfmoe_permute_workspace_bytes(T, k, n_experts))
+    # one allocation: offsets, counts, perm_tok, pos_of, workspace
+    n = T * k
+    buf = torch.empty(2 * n_experts + 1 + 2 * n + ws_bytes // 4, dtype=torch.int32, device=idx.device)
+    offsets, counts, perm_tok, pos_of, ws = buf.split_with_sizes([n_experts + 1, n_experts, n, n, ws_bytes // 4])
+    check(lib.vfmoe_permute(_ptr(idx), T, k, n_experts, _ptr(x), dt, H, _ptr(xs), _ptr(counts), _ptr(offsets),
+                            _ptr(perm_tok), _ptr(pos_of), _ptr(ws), ws_bytes, _stream()))
+    return xs, Plan(perm_tok, pos_of, offsets, counts)
+
+
+def permute_backward(dxs: torch.Tensor, pos_of: torch.Tensor, T: int, k: int, out_dtype=None) -> torch.Tensor:
+    """dx [T, H] from the gradient dxs of permute's rows: the sum over each token's lanes
+    (vfmoe_permute_backward), of dxs's dtype unless out_dtype names another."""
+    _check(dxs, "dxs", _FLOATS, (-1, -1))
+    _check(pos_of, "pos_of", _I32, (T * k,))
+    H = dxs.shape[1]
+    out_dtype = out_dtype or dxs.dtype
+    _need(out_dtype in _DT, f"out_dtype {out_dtype} is not supported")
+    dx = torch.empty((T, H), dtype=out_dtype, device=dxs.device)
+    check(_lib.load().vfmoe_permute_backward(_ptr(dxs), _DT[dxs.dtype], _ptr(pos_of), T, k, H, _ptr(dx),
+                                             _DT[dx.dtype], _stream()))
+    return dx
+
+
 def combine(y: torch.Tensor, pos_of: torch.Tensor, w, T: int, k: int, y_shared=None,
             out_dtype=torch.bfloat16) -> torch.Tensor:
-    """out[t] = sum_l w[t,l] * y[pos_of[t*k+l]] (+ y_shared[t]); y fp32 or fp16; pos < 0 skips."""
+    """out[t] = sum_l w[t,l] * y[pos_of[t*k+l]] (+ y_shared[t]); y fp32, fp16 or bf16; pos < 0 skips."""
+    _check(y, "y", _FLOATS, (-1, -1))
     H = y.shape[1]
-    out = torch.empty((T, H), dtype=out_dtype, device=y.device)
+    _need(pos_of.dtype == torch.int32 and pos_of.is_contiguous() and pos_of.numel() >= T * k,
+          f"pos_of: {T * k} contiguous int32 positions are needed")
+    _need(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() >= T * k),
+          f"w: {T * k} contiguous fp32 weights are needed")
+    _need(out_dtype in _DT, f"out_dtype {out_dtype} is not supported")
     if y_shared is not None:
-        assert y_shared.dtype == y.dtype
+        _check(y_shared, "y_shared", (y.dtype,), (T, H))
+    out = torch.empty((T, H), dtype=out_dtype, device=y.device)
     check(_lib.load().vfmoe_combine(_ptr(y), _DT[y.dtype], _ptr(pos_of), _ptr(w), T, k, H, _ptr(y_shared), _ptr(out),
                                     _DT[out_dtype], _stream()))
     return out
+
+
+def combine_backward(dout: torch.Tensor, y: torch.Tensor, pos_of: torch.Tensor, w: torch.Tensor | None, T: int, k: int,
+                     dy: torch.Tensor | None = None):
+    """(dy, dw fp32 [T, k]) of combine from dout [T, H] (vfmoe_combine_backward).  dy has y's shape and dtype
+    and may be y itself; its rows that no lane names stay as they were (undefined when `dy` is not given).
+    The gradient of combine's y_shared is dout."""
+    _check(y, "y", _FLOATS, (-1, -1))
+    H = y.shape[1]
+    _check(dout, "dout", _FLOATS, (T, H))
+    _check(pos_of, "pos_of", _I32, (T * k,))
+    if w is not None:
+        _check(w, "w", _F32, (T, k))
+    if dy is None:
+        dy = torch.empty_like(y)
+    else:
+        _check(dy, "dy", (y.dtype,), y.shape)
+    dw = torch.empty((T, k), dtype=torch.float32, device=y.device)
+    check(_lib.load().vfmoe_combine_backward(_ptr(dout), _DT[dout.dtype], _ptr(y), _DT[y.dtype], _ptr(pos_of), _ptr(w),
+                                             T, k, H, _ptr(dy), _ptr(dw), _stream()))
+    return dy, dw
 
 
 def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
