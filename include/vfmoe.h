@@ -234,12 +234,9 @@ int vfmoe_combine_backward(int64_t dout, int64_t dout_dtype, int64_t y, int64_t 
  * error here.  A token may name one expert on several lanes; rows are ordered by (expert, token, lane).
  *   counts [n_experts], offsets [n_experts + 1], perm_tok [T*k], pos_of [T*k]: as vfmoe_dispatch;
  *   perm_tok is -1 from row offsets[n_experts] on, and those rows of xs stay as they were.
- * x = 0 makes the plan alone.  n_experts <= 1024, k <= 32, T*k <= 2^30.  workspace: at least
- * vfmoe_permute_workspace_bytes (0 for decode batches); calls that overlap on the GPU need one each. */
-int64_t vfmoe_permute_workspace_bytes(int64_t T, int64_t k, int64_t n_experts);
+ * x = 0 makes the plan alone.  n_experts <= 1024, k <= 32, T*k <= 2^30. */
 int vfmoe_permute(int64_t idx, int64_t T, int64_t k, int64_t n_experts, int64_t x, int64_t dtype, int64_t H,
-                  int64_t xs, int64_t counts, int64_t offsets, int64_t perm_tok, int64_t pos_of, int64_t workspace,
-                  int64_t ws_bytes, int64_t stream);
+                  int64_t xs, int64_t counts, int64_t offsets, int64_t perm_tok, int64_t pos_of, int64_t stream);
 
 /* Gradient of the sorted rows: dx[t] = sum over the token's lanes with a row of dxs[pos_of[t*k+l]], in
  * lane order in fp32, rounded once to dx_dtype (a token without rows gets zeros). */

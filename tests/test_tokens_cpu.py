@@ -8,8 +8,8 @@ from vybforge_b200 import _lib
 A = 1 << 20  # a well-aligned address
 
 
-def permute(lib, idx=A, T=4, k=2, E=16, x=A, dt=0, H=64, xs=A, counts=A, offsets=A, perm=A, pos=A, ws=0, wsb=0):
-    return lib.vfmoe_permute(idx, T, k, E, x, dt, H, xs, counts, offsets, perm, pos, ws, wsb, 0)
+def permute(lib, idx=A, T=4, k=2, E=16, x=A, dt=0, H=64, xs=A, counts=A, offsets=A, perm=A, pos=A):
+    return lib.vfmoe_permute(idx, T, k, E, x, dt, H, xs, counts, offsets, perm, pos, 0)
 
 
 @pytest.mark.parametrize("kw", [dict(idx=0), dict(T=-1), dict(k=0), dict(k=33), dict(E=0), dict(E=1025), dict(dt=3),
@@ -19,16 +19,6 @@ def permute(lib, idx=A, T=4, k=2, E=16, x=A, dt=0, H=64, xs=A, counts=A, offsets
 def test_permute_refuses(built_lib, kw):
     assert permute(built_lib, **kw) == _lib.ERR_INVALID
     assert "vfmoe_permute" in _lib.last_error()
-
-
-def test_permute_workspace(built_lib):
-    assert built_lib.vfmoe_permute_workspace_bytes(4, 2, 16) == 0
-    need = built_lib.vfmoe_permute_workspace_bytes(8192, 8, 256)
-    assert need == 64 * 256 * 4
-    assert built_lib.vfmoe_permute_workspace_bytes(4, 2, 0) == _lib.ERR_INVALID
-    assert built_lib.vfmoe_permute_workspace_bytes(-1, 2, 4) == _lib.ERR_INVALID
-    assert permute(built_lib, T=8192, k=8, E=256) == _lib.ERR_WORKSPACE
-    assert permute(built_lib, T=8192, k=8, E=256, ws=A, wsb=need - 1) == _lib.ERR_WORKSPACE
 
 
 @pytest.mark.parametrize("kw", [dict(y=0), dict(dt=5), dict(pos=0), dict(T=-2), dict(k=0), dict(k=40), dict(H=0),

@@ -101,8 +101,7 @@ _SIGS = {
     "vfmoe_forward_rows": (C.c_int, [I64] * 9),
     "vfmoe_combine": (C.c_int, [I64] * 11),
     "vfmoe_combine_backward": (C.c_int, [I64] * 12),
-    "vfmoe_permute_workspace_bytes": (I64, [I64] * 3),
-    "vfmoe_permute": (C.c_int, [I64] * 15),
+    "vfmoe_permute": (C.c_int, [I64] * 13),
     "vfmoe_permute_backward": (C.c_int, [I64] * 9),
     "vfmoe_routed_workspace_bytes": (I64, [I64, I64, I64]),
     "vfmoe_forward_routed": (C.c_int, [I64] * 12),

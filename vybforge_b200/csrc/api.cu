@@ -758,28 +758,13 @@ int vfmoe_combine_backward(int64_t dout, int64_t dout_dtype, int64_t y, int64_t 
                                    reinterpret_cast<cudaStream_t>(stream));
 }
 
-int64_t vfmoe_permute_workspace_bytes(int64_t T, int64_t k, int64_t n_experts) {
-    if (!lanes_ok(T, k, 1) || n_experts <= 0 || n_experts > 1024) {
-        set_error("vfmoe_permute_workspace_bytes: bad arguments");
-        return VFMOE_ERR_INVALID;
-    }
-    return permute_ws_bytes(T, (int)k, (int)n_experts);
-}
-
 int vfmoe_permute(int64_t idx, int64_t T, int64_t k, int64_t n_experts, int64_t x, int64_t dtype, int64_t H,
-                  int64_t xs, int64_t counts, int64_t offsets, int64_t perm_tok, int64_t pos_of, int64_t workspace,
-                  int64_t ws_bytes, int64_t stream) {
+                  int64_t xs, int64_t counts, int64_t offsets, int64_t perm_tok, int64_t pos_of, int64_t stream) {
     if (!lanes_ok(T, k, x ? H : 1) || n_experts <= 0 || n_experts > 1024 || !counts || !offsets ||
-        (T > 0 && (!idx || !perm_tok || !pos_of)) || (idx | counts | offsets | perm_tok | pos_of | workspace) % 4 ||
+        (T > 0 && (!idx || !perm_tok || !pos_of)) || (idx | counts | offsets | perm_tok | pos_of) % 4 ||
         (x && (!is_float_dtype(dtype) || !xs || (x | xs) % dtype_bytes(dtype)))) {
         set_error("vfmoe_permute: bad arguments");
         return VFMOE_ERR_INVALID;
-    }
-    const int64_t need = permute_ws_bytes(T, (int)k, (int)n_experts);
-    if (need && (!workspace || ws_bytes < need)) {
-        set_error("vfmoe_permute: workspace of %lld bytes, %lld needed", (long long)(workspace ? ws_bytes : 0),
-                  (long long)need);
-        return VFMOE_ERR_WORKSPACE;
     }
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     if (T == 0) {
@@ -790,8 +775,7 @@ int vfmoe_permute(int64_t idx, int64_t T, int64_t k, int64_t n_experts, int64_t 
     return launch_permute(reinterpret_cast<const int32_t *>(idx), T, (int)k, (int)n_experts,
                           reinterpret_cast<const void *>(x), (int)dtype, H, reinterpret_cast<void *>(xs),
                           reinterpret_cast<int32_t *>(counts), reinterpret_cast<int32_t *>(offsets),
-                          reinterpret_cast<int32_t *>(perm_tok), reinterpret_cast<int32_t *>(pos_of),
-                          reinterpret_cast<int32_t *>(workspace), st);
+                          reinterpret_cast<int32_t *>(perm_tok), reinterpret_cast<int32_t *>(pos_of), st);
 }
 
 int vfmoe_permute_backward(int64_t dxs, int64_t dtype, int64_t pos_of, int64_t T, int64_t k, int64_t H, int64_t dx,

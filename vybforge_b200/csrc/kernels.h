@@ -74,11 +74,9 @@ int launch_gather(const void *x, int x_dtype, const int32_t *perm_tok, int64_t r
 int launch_combine(const void *y, int y_dtype, const int32_t *pos_of, const float *w, int T, int H, int k,
                    const void *y_shared, void *out, int out_dtype, cudaStream_t st);
 // Sorted tokens in the caller's element type, the way back and the gradients (tokens.cu).
-// launch_permute: ws of permute_ws_bytes; x = 0: the plan only.
-int64_t permute_ws_bytes(int64_t T, int k, int E);
+// launch_permute with x = 0: the plan only.
 int launch_permute(const int32_t *idx, int64_t T, int k, int E, const void *x, int dtype, int64_t H, void *xs,
-                   int32_t *counts, int32_t *offsets, int32_t *perm_tok, int32_t *pos_of, int32_t *ws,
-                   cudaStream_t st);
+                   int32_t *counts, int32_t *offsets, int32_t *perm_tok, int32_t *pos_of, cudaStream_t st);
 int launch_return_rows(const void *y, int y_dtype, const int32_t *pos_of, const float *w, int64_t T, int64_t H, int k,
                        const void *y_shared, void *out, int out_dtype, cudaStream_t st);
 int launch_combine_backward(const void *dout, int dout_dtype, const void *y, int y_dtype, const int32_t *pos_of,
