@@ -478,6 +478,37 @@ int vfmoe_q8_0_quantize(int64_t src_f32, int64_t dst, int64_t rows, int64_t k, i
  * reference (a load-time layout step; its kernels read GGUF rows in place). */
 int vfmoe_q8_0_tile(int64_t src, int64_t dst, int64_t rows, int64_t k, int64_t n_mats, int64_t stream);
 
+/* ---- 4-bit matrices with group scales (no counterpart in the reference, whose linear 4-bit weights are GGUF
+ * types it does not run on the GPU): n_mats matrices [n][k], rows = output channels, w = s * (q - z) ----
+ *   data    uint8 [n_mats][n][k/2]: codes 0..15, element 2j of a row in the low nibble of byte j
+ *   scales  fp16 or bf16 (scale_dtype) [n_mats][k/group][n]: a group is `group` consecutive elements of a row
+ *   zeros   uint8 [n_mats][k/group][n], zero points 0..15 one a byte (the low four bits count); 0: all are 8
+ * n a multiple of 16, group 32, 64 or 128, k a multiple of group, n_mats <= 1024, 16-byte aligned addresses. */
+typedef struct vfmoe_q4_matrix {
+    int64_t n, k, group, n_mats, scale_dtype;
+    int64_t data, scales, zeros;
+} vfmoe_q4_matrix;
+
+/* Products of 4-bit matrices with a few rows (decode batches; more rows run in tiles):
+ *   y[r] = W x[row_map ? row_map[r] : r]            x [x_rows][k], y [rows][n], any of F32, F16, BF16
+ * offsets = 0: one matrix.  Else int32 [n_mats + 1] (vfmoe_permute, vfmoe_dispatch): rows [offsets[e],
+ * offsets[e+1]) belong to matrix e, `rows` bounds offsets[n_mats], and rows of y from offsets[n_mats] on
+ * stay as they were.  With the plan's perm_tok as row_map the unsorted rows are read in place.  A row_map
+ * entry outside [0, x_rows) reads as a row of zeros.
+ * up != 0: a second matrix of the same kind, y = silu(min(W x, limit)) * clip(up x, -limit, limit)
+ * (moe_ref.py:81-84; limit > 0, infinity for none).  q - z is exact in the tensor cores' operands, and so is x (fp32
+ * x as three bf16 parts): sums, the group scales and the SwiGLU are fp32, one rounding to y_dtype. */
+int vfmoe_q4_matvec(const vfmoe_q4_matrix *w, const vfmoe_q4_matrix *up, double limit, int64_t x, int64_t x_dtype,
+                    int64_t x_rows, int64_t row_map, int64_t offsets, int64_t rows, int64_t y, int64_t y_dtype,
+                    int64_t stream);
+
+/* [n_mats][n][k] values (F32, F16 or BF16, finite) -> dst's buffers, round to nearest.  Without zeros s =
+ * max|w| / 7; with zeros the range of the group and 0 in 15 steps.  The scale is rounded to scale_dtype first. */
+int vfmoe_q4_quantize(int64_t src, int64_t src_dtype, const vfmoe_q4_matrix *dst, int64_t stream);
+
+/* 4-bit matrices -> dense [n_mats][n][k] (F32, F16 or BF16): the fp32 product s * (q - z), rounded once. */
+int vfmoe_q4_dequant(const vfmoe_q4_matrix *src, int64_t dst, int64_t dst_dtype, int64_t stream);
+
 /* EXL3 trellis -> rotated-basis values W^ as fp16 [K, N] (no Hadamard).
  * Replaces exl3deq / exl3deq32 (native/kernels/exl3.vyb:207-242,375-422).
  * bits = 3 (layout defined by this library) or 4 (the reference's format: its slot map,

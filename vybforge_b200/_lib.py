@@ -56,6 +56,11 @@ class LayerDesc(C.Structure):
                 ("expert_path", C.c_int64), ("shared_format", C.c_int64)]
 
 
+class Q4Desc(C.Structure):
+    _fields_ = [("n", C.c_int64), ("k", C.c_int64), ("group", C.c_int64), ("n_mats", C.c_int64),
+                ("scale_dtype", C.c_int64), ("data", C.c_int64), ("scales", C.c_int64), ("zeros", C.c_int64)]
+
+
 class HcDesc(C.Structure):
     _fields_ = [("n_streams", C.c_int64), ("hidden", C.c_int64), ("fn", C.c_int64), ("fn_dtype", C.c_int64),
                 ("base", C.c_int64), ("scale", C.c_int64), ("rms_eps", C.c_double), ("hc_eps", C.c_double),
@@ -121,6 +126,9 @@ _SIGS = {
     "vfmoe_q8_0_dequant": (C.c_int, [I64] * 6),
     "vfmoe_q8_0_quantize": (C.c_int, [I64] * 5),
     "vfmoe_q8_0_tile": (C.c_int, [I64] * 6),
+    "vfmoe_q4_matvec": (C.c_int, [C.POINTER(Q4Desc), C.POINTER(Q4Desc), C.c_double] + [I64] * 9),
+    "vfmoe_q4_quantize": (C.c_int, [I64, I64, C.POINTER(Q4Desc), I64]),
+    "vfmoe_q4_dequant": (C.c_int, [C.POINTER(Q4Desc), I64, I64, I64]),
     "vfmoe_exl3_decode": (C.c_int, [I64] * 6),
 }
 

@@ -21,6 +21,7 @@
 #include "kernels.h"
 #include "expert_tc.h"
 #include "layer.h"
+#include "q4.h"
 
 namespace vfmoe {
 
@@ -955,6 +956,83 @@ int vfmoe_q8_0_tile(int64_t src, int64_t dst, int64_t rows, int64_t k, int64_t n
     }
     return launch_q8_0_tile(reinterpret_cast<const uint8_t *>(src), reinterpret_cast<uint8_t *>(dst), rows, k,
                             n_mats, reinterpret_cast<cudaStream_t>(stream));
+}
+
+static bool q4_ok(const vfmoe_q4_matrix *m, const char *who) {
+    if (!m || m->n <= 0 || m->n % 16 || m->n > ((int64_t)1 << 24) || m->k <= 0 || m->k > ((int64_t)1 << 24) ||
+        (m->group != 32 && m->group != 64 && m->group != 128) || m->k % m->group || m->n_mats <= 0 ||
+        m->n_mats > 1024 || (m->scale_dtype != VFMOE_DT_F16 && m->scale_dtype != VFMOE_DT_BF16) || !m->data ||
+        !m->scales || (m->data | m->scales | m->zeros) & 15) {
+        set_error("%s: bad 4-bit matrix (n a multiple of 16, k of group, group 32, 64 or 128, at most 1024 matrices, "
+                  "fp16 or bf16 scales, 16-byte aligned)", who);
+        return false;
+    }
+    return true;
+}
+
+static Q4Mat q4_mat(const vfmoe_q4_matrix &m) {
+    return Q4Mat{reinterpret_cast<const uint8_t *>(m.data), reinterpret_cast<const uint16_t *>(m.scales),
+                 reinterpret_cast<const uint8_t *>(m.zeros)};
+}
+
+int vfmoe_q4_quantize(int64_t src, int64_t src_dtype, const vfmoe_q4_matrix *dst, int64_t stream) {
+    if (!q4_ok(dst, "vfmoe_q4_quantize")) return VFMOE_ERR_INVALID;
+    if (!is_float_dtype(src_dtype) || !src || src % dtype_bytes(src_dtype)) {
+        set_error("vfmoe_q4_quantize: bad arguments");
+        return VFMOE_ERR_INVALID;
+    }
+    return launch_q4_quantize(reinterpret_cast<const void *>(src), (int)src_dtype, dst->n, dst->k, (int)dst->group,
+                              dst->n_mats, reinterpret_cast<uint8_t *>(dst->data),
+                              reinterpret_cast<uint16_t *>(dst->scales), dst->scale_dtype == VFMOE_DT_F16,
+                              reinterpret_cast<uint8_t *>(dst->zeros), reinterpret_cast<cudaStream_t>(stream));
+}
+
+int vfmoe_q4_dequant(const vfmoe_q4_matrix *src, int64_t dst, int64_t dst_dtype, int64_t stream) {
+    if (!q4_ok(src, "vfmoe_q4_dequant")) return VFMOE_ERR_INVALID;
+    if (!is_float_dtype(dst_dtype) || !dst || dst % dtype_bytes(dst_dtype)) {
+        set_error("vfmoe_q4_dequant: bad arguments");
+        return VFMOE_ERR_INVALID;
+    }
+    return launch_q4_dequant(q4_mat(*src), src->n, src->k, (int)src->group, src->n_mats,
+                             src->scale_dtype == VFMOE_DT_F16, reinterpret_cast<void *>(dst), (int)dst_dtype,
+                             reinterpret_cast<cudaStream_t>(stream));
+}
+
+int vfmoe_q4_matvec(const vfmoe_q4_matrix *w, const vfmoe_q4_matrix *up, double limit, int64_t x, int64_t x_dtype,
+                    int64_t x_rows, int64_t row_map, int64_t offsets, int64_t rows, int64_t y, int64_t y_dtype,
+                    int64_t stream) {
+    if (!q4_ok(w, "vfmoe_q4_matvec") || (up && !q4_ok(up, "vfmoe_q4_matvec"))) return VFMOE_ERR_INVALID;
+    if (up && (up->n != w->n || up->k != w->k || up->group != w->group || up->n_mats != w->n_mats ||
+               up->scale_dtype != w->scale_dtype || !up->zeros != !w->zeros || !(limit > 0))) {
+        set_error("vfmoe_q4_matvec: up must have the shape, group, scale type and kind of zero points of the gate, and "
+                  "limit must be positive");
+        return VFMOE_ERR_INVALID;
+    }
+    if (!is_float_dtype(x_dtype) || !is_float_dtype(y_dtype) || rows < 0 || rows > ((int64_t)1 << 30) || x_rows < 0 ||
+        x_rows > ((int64_t)1 << 30) || (!offsets && w->n_mats != 1) || (!row_map && x_rows < rows) ||
+        (rows > 0 && (!x || !y)) || (x | y) & 15 || (row_map | offsets) % 4) {
+        set_error("vfmoe_q4_matvec: bad arguments (16-byte aligned x and y, x_rows >= rows without a row map, offsets "
+                  "for more than one matrix)");
+        return VFMOE_ERR_INVALID;
+    }
+    if (rows == 0) return VFMOE_OK;
+    Q4Args a{};
+    a.N = w->n;
+    a.K = w->k;
+    a.G = (int)w->group;
+    a.E = (int)w->n_mats;
+    a.scale_f16 = w->scale_dtype == VFMOE_DT_F16;
+    a.w = q4_mat(*w);
+    if (up) a.up = q4_mat(*up);
+    a.limit = (float)limit;
+    a.x = reinterpret_cast<const void *>(x);
+    a.x_rows = x_rows;
+    a.row_map = reinterpret_cast<const int32_t *>(row_map);
+    a.offsets = reinterpret_cast<const int32_t *>(offsets);
+    a.rows = rows;
+    a.y = reinterpret_cast<void *>(y);
+    a.y_dtype = (int)y_dtype;
+    return launch_q4_matvec(a, (int)x_dtype, reinterpret_cast<cudaStream_t>(stream));
 }
 
 int vfmoe_exl3_decode(int64_t trellis, int64_t dst_f16, int64_t K, int64_t N, int64_t bits, int64_t stream) {

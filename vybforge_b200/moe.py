@@ -378,6 +378,76 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, pos_of: torch.Tensor, 
     return dy, dw
 
 
+class Q4Matrix:
+    """4-bit matrices with group scales (vfmoe_q4_matrix): codes uint8 [N, K/2] (element 2j of a row in the low
+    nibble of byte j), scales fp16 or bf16 [K/G, N], zeros uint8 [K/G, N] or None (8): w = s * (q - z).  Stacked
+    matrices have a leading dimension E.  N % 16 == 0, G in {32, 64, 128}."""
+
+    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None = None):
+        lead = (-1,) * (codes.dim() - 2)
+        _need(codes.dim() in (2, 3), "codes: [N, K/2] or [E, N, K/2]")
+        _check(codes, "codes", (torch.uint8,), lead + (-1, -1))
+        N, K = codes.shape[-2], 2 * codes.shape[-1]
+        _check(scales, "scales", (torch.float16, torch.bfloat16), tuple(codes.shape[:-2]) + (-1, N))
+        if zeros is not None:
+            _check(zeros, "zeros", (torch.uint8,), scales.shape)
+        groups = scales.shape[-2]
+        _need(groups > 0 and K % groups == 0, f"scales: {groups} groups do not divide K = {K}")
+        self.codes, self.scales, self.zeros = codes, scales, zeros
+        self.N, self.K, self.group = N, K, K // groups
+        self.n_mats = codes.shape[0] if lead else 1
+        self.desc = _lib.Q4Desc(N, K, self.group, self.n_mats, _DT[scales.dtype], _ptr(codes), _ptr(scales),
+                                _ptr(zeros))
+
+
+def q4_quantize(w: torch.Tensor, group: int = 128, scale_dtype=torch.bfloat16, zeros: bool = False) -> Q4Matrix:
+    """4-bit codes of w [N, K] or [E, N, K], round to nearest (vfmoe_q4_quantize)."""
+    _need(w.dim() in (2, 3), "w: [N, K] or [E, N, K]")
+    _check(w, "w", _FLOATS, (-1,) * w.dim())
+    N, K = w.shape[-2:]
+    _need(group in (32, 64, 128) and K % group == 0 and K > 0, f"group = {group}: 32, 64 or 128, and a divisor of K = {K}")
+    lead = tuple(w.shape[:-2])
+    m = Q4Matrix(w.new_empty(lead + (N, K // 2), dtype=torch.uint8),
+                 w.new_empty(lead + (K // group, N), dtype=scale_dtype),
+                 w.new_empty(lead + (K // group, N), dtype=torch.uint8) if zeros else None)
+    check(_lib.load().vfmoe_q4_quantize(_ptr(w), _DT[w.dtype], C.byref(m.desc), _stream()))
+    return m
+
+
+def q4_dequant(w: Q4Matrix, dtype=torch.float32) -> torch.Tensor:
+    """Dense [N, K] or [E, N, K] of 4-bit matrices (vfmoe_q4_dequant)."""
+    _need(dtype in _DT, f"dtype {dtype} is not supported")
+    out = w.codes.new_empty(tuple(w.codes.shape[:-1]) + (w.K,), dtype=dtype)
+    check(_lib.load().vfmoe_q4_dequant(C.byref(w.desc), _ptr(out), _DT[dtype], _stream()))
+    return out
+
+
+def q4_matvec(x: torch.Tensor, w: Q4Matrix, up: Q4Matrix | None = None, limit: float = 10.0,
+              offsets: torch.Tensor | None = None, row_map: torch.Tensor | None = None,
+              out: torch.Tensor | None = None, out_dtype=None) -> torch.Tensor:
+    """y [R, N] = the rows of x [.., K] times w^T (vfmoe_q4_matvec).  offsets int32 [E + 1]: the rows are sorted
+    by matrix (permute's plan); row_map int32 [R]: the row of x of each row of y (the plan's perm_tok reads the
+    unsorted rows).  up: gate and up products and their clamped SwiGLU.  Rows of y behind offsets[-1] stay as they
+    were (undefined when `out` is not given)."""
+    _check(x, "x", _FLOATS, (-1, w.K))
+    R = x.shape[0]
+    if row_map is not None:
+        _check(row_map, "row_map", _I32, (-1,))
+        R = row_map.shape[0]
+    if offsets is not None:
+        _check(offsets, "offsets", _I32, (w.n_mats + 1,))
+    if out is None:
+        out_dtype = out_dtype or x.dtype
+        _need(out_dtype in _DT, f"out_dtype {out_dtype} is not supported")
+        out = x.new_empty((R, w.N), dtype=out_dtype)
+    else:
+        _check(out, "out", _FLOATS if out_dtype is None else (out_dtype,), (R, w.N))
+    check(_lib.load().vfmoe_q4_matvec(C.byref(w.desc), None if up is None else C.byref(up.desc), limit, _ptr(x),
+                                      _DT[x.dtype], x.shape[0], _ptr(row_map), _ptr(offsets), R, _ptr(out),
+                                      _DT[out.dtype], _stream()))
+    return out
+
+
 def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
     y = torch.empty_like(x)
     S, D = x.shape
