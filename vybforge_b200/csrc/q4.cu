@@ -1,4 +1,4 @@
-// 4-bit matrices with group scales: quantize, dequantize, and products with a few rows.
+// 4-bit matrices with group scales: quantize and dequantize (the products: q4_matvec.cuh).
 #include "common.cuh"
 #include "q4.h"
 
@@ -63,51 +63,10 @@ __global__ void __launch_bounds__(256) q4_dequant_kernel(Q4Mat w, int64_t N, int
     st_act(dst, 2 * i + 1, s * (float)((b >> 4) - z), dst_dtype);
 }
 
-// One warp an output channel of one row: lane l adds the bytes l, l + 32, ... of the row.
-__global__ void __launch_bounds__(256) q4_matvec_simple_kernel(Q4Args a, int x_dtype) {
-    const int lane = threadIdx.x & 31;
-    const int64_t n = blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (n >= a.N) return;
-    for (int64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        int64_t e = 0;
-        if (a.offsets) {
-            if (r >= a.offsets[a.E]) return;
-            int lo = 0, hi = a.E;  // offsets[lo] <= r < offsets[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) / 2;
-                if (a.offsets[mid] <= r) lo = mid;
-                else hi = mid;
-            }
-            e = lo;
-        }
-        const int64_t xr = a.row_map ? a.row_map[r] : r;
-        float sum[2] = {0.f, 0.f};
-        for (int p = 0; p < (a.up.data ? 2 : 1); ++p) {
-            const Q4Mat &w = p ? a.up : a.w;
-            for (int64_t b = lane; b < a.K / 2 && xr >= 0 && xr < a.x_rows; b += 32) {
-                const int64_t sz = (e * (a.K / a.G) + 2 * b / a.G) * a.N + n;
-                const int z = w.zeros ? w.zeros[sz] & 15 : 8;
-                const int c = w.data[(e * a.N + n) * (a.K / 2) + b];
-                const float t = (float)((c & 15) - z) * ld_act(a.x, xr * a.K + 2 * b, x_dtype) +
-                                (float)((c >> 4) - z) * ld_act(a.x, xr * a.K + 2 * b + 1, x_dtype);
-                sum[p] = fmaf(q4_scale(w.scales[sz], a.scale_f16), t, sum[p]);
-            }
-            sum[p] = warp_sum_f32(sum[p]);
-        }
-        if (lane == 0) {
-            const float v = a.up.data ? swiglu_clamped(sum[0], sum[1], a.limit) : sum[0];
-            st_act(a.y, r * a.N + n, v, a.y_dtype);
-        }
-    }
-}
-
 }  // namespace
 
 int launch_q4_matvec(const Q4Args &a, int x_dtype, cudaStream_t st) {
-    const int64_t rows = a.rows < 65535 ? a.rows : 65535;
-    q4_matvec_simple_kernel<<<dim3((unsigned)cdiv(a.N, 8), (unsigned)rows), 256, 0, st>>>(a, x_dtype);
-    VF_LAUNCH_CHECK("q4_matvec_simple_kernel");
-    return VFMOE_OK;
+    return x_dtype == VFMOE_DT_BF16 ? launch_q4_bf16(a, st) : x_dtype == VFMOE_DT_F16 ? launch_q4_f16(a, st) : launch_q4_f32(a, st);
 }
 
 int launch_q4_quantize(const void *src, int src_dtype, int64_t N, int64_t K, int G, int64_t n_mats, uint8_t *data,

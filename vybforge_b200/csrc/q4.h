@@ -31,6 +31,10 @@ struct Q4Args {
 };
 
 int launch_q4_matvec(const Q4Args &a, int x_dtype, cudaStream_t st);
+// one translation unit a type of x (q4_bf16.cu, q4_f16.cu, q4_f32.cu)
+int launch_q4_bf16(const Q4Args &a, cudaStream_t st);
+int launch_q4_f16(const Q4Args &a, cudaStream_t st);
+int launch_q4_f32(const Q4Args &a, cudaStream_t st);
 int launch_q4_quantize(const void *src, int src_dtype, int64_t N, int64_t K, int G, int64_t n_mats, uint8_t *data,
                        uint16_t *scales, int scale_f16, uint8_t *zeros, cudaStream_t st);
 int launch_q4_dequant(const Q4Mat &w, int64_t N, int64_t K, int G, int64_t n_mats, int scale_f16, void *dst,
