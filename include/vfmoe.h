@@ -224,7 +224,8 @@ int vfmoe_combine(int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w, int64_t
  *   dy[pos] = w[t,l] * dout[t]        (y_dtype, one rounding; rows that no lane names stay as they were)
  *   dw[t,l] = <dout[t], y[pos]>       (fp32; 0 for a lane without a row)
  * dy or dw may be 0 (y is read for dw only); w = 0: weight 1; dy may be y itself.  The gradient of
- * y_shared is dout.  No counterpart in the reference, whose MoE path is forward only. */
+ * y_shared is dout.  The positions are those of a plan: no two lanes name one row.  No counterpart in the
+ * reference, whose MoE path is forward only. */
 int vfmoe_combine_backward(int64_t dout, int64_t dout_dtype, int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w,
                            int64_t T, int64_t k, int64_t H, int64_t dy, int64_t dw, int64_t stream);
 
@@ -234,6 +235,7 @@ int vfmoe_combine_backward(int64_t dout, int64_t dout_dtype, int64_t y, int64_t 
  * error here.  A token may name one expert on several lanes; rows are ordered by (expert, token, lane).
  *   counts [n_experts], offsets [n_experts + 1], perm_tok [T*k], pos_of [T*k]: as vfmoe_dispatch;
  *   perm_tok is -1 from row offsets[n_experts] on, and those rows of xs stay as they were.
+ * xs must not overlap x.
  * x = 0 makes the plan alone.  n_experts <= 1024, k <= 32, T*k <= 2^30. */
 int vfmoe_permute(int64_t idx, int64_t T, int64_t k, int64_t n_experts, int64_t x, int64_t dtype, int64_t H,
                   int64_t xs, int64_t counts, int64_t offsets, int64_t perm_tok, int64_t pos_of, int64_t stream);
@@ -494,7 +496,7 @@ typedef struct vfmoe_q4_matrix {
  * offsets = 0: one matrix.  Else int32 [n_mats + 1] (vfmoe_permute, vfmoe_dispatch): rows [offsets[e],
  * offsets[e+1]) belong to matrix e, `rows` bounds offsets[n_mats], and rows of y from offsets[n_mats] on
  * stay as they were.  With the plan's perm_tok as row_map the unsorted rows are read in place.  A row_map
- * entry outside [0, x_rows) reads as a row of zeros.
+ * entry outside [0, x_rows) reads as a row of zeros.  y must not overlap x.
  * up != 0: a second matrix of the same kind, y = silu(min(W x, limit)) * clip(up x, -limit, limit)
  * (moe_ref.py:81-84; limit > 0, infinity for none).  q - z is exact in the tensor cores' operands, and so is x (fp32
  * x as three bf16 parts): sums, the group scales and the SwiGLU are fp32, one rounding to y_dtype. */

@@ -166,6 +166,8 @@ def test_row_map_outside_reads_zeros():
     ref = moe.q4_matvec(x, m)
     for r, i in enumerate(at.tolist()):
         assert torch.equal(y[r], ref[i] if 0 <= i < 4 else torch.zeros_like(ref[0]))
+    none = moe.q4_matvec(x[:0], m, row_map=torch.full((3,), -1, dtype=torch.int32, device="cuda"))
+    assert none.shape == (3, 32) and bool((none == 0).all())
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

@@ -318,6 +318,8 @@ def test_refusals():
         lambda: moe.combine(y[:, ::2], pos, w, 4, 2),
         lambda: moe.combine(y, pos[:7], w, 4, 2),
         lambda: moe.combine(y, pos, w.half(), 4, 2),
+        lambda: moe.combine(y, pos, w.cpu(), 4, 2),
+        lambda: moe.combine(y, pos.cpu(), w, 4, 2),
         lambda: moe.combine(y, pos, w, 4, 2, y_shared=x.half()),
         lambda: moe.combine(y, pos, w, 4, 2, out_dtype=torch.float64),
         lambda: moe.combine_backward(x[:3], y, pos, w, 4, 2),

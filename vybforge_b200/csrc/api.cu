@@ -1010,7 +1010,7 @@ int vfmoe_q4_matvec(const vfmoe_q4_matrix *w, const vfmoe_q4_matrix *up, double 
     }
     if (!is_float_dtype(x_dtype) || !is_float_dtype(y_dtype) || rows < 0 || rows > ((int64_t)1 << 30) || x_rows < 0 ||
         x_rows > ((int64_t)1 << 30) || (!offsets && w->n_mats != 1) || (!row_map && x_rows < rows) ||
-        (rows > 0 && (!x || !y)) || (x | y) & 15 || (row_map | offsets) % 4) {
+        (rows > 0 && ((!x && x_rows > 0) || !y)) || (x | y) & 15 || (row_map | offsets) % 4) {
         set_error("vfmoe_q4_matvec: bad arguments (16-byte aligned x and y, x_rows >= rows without a row map, offsets "
                   "for more than one matrix)");
         return VFMOE_ERR_INVALID;

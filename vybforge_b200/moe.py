@@ -344,10 +344,11 @@ def combine(y: torch.Tensor, pos_of: torch.Tensor, w, T: int, k: int, y_shared=N
     """out[t] = sum_l w[t,l] * y[pos_of[t*k+l]] (+ y_shared[t]); y fp32, fp16 or bf16; pos < 0 skips."""
     _check(y, "y", _FLOATS, (-1, -1))
     H = y.shape[1]
-    _need(pos_of.dtype == torch.int32 and pos_of.is_contiguous() and pos_of.numel() >= T * k,
-          f"pos_of: {T * k} contiguous int32 positions are needed")
-    _need(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() >= T * k),
-          f"w: {T * k} contiguous fp32 weights are needed")
+    dev = y.get_device()
+    _need(pos_of.dtype == torch.int32 and pos_of.is_contiguous() and pos_of.numel() >= T * k and
+          pos_of.get_device() == dev, f"pos_of: {T * k} contiguous int32 positions on y's device are needed")
+    _need(w is None or (w.dtype == torch.float32 and w.is_contiguous() and w.numel() >= T * k and
+                        w.get_device() == dev), f"w: {T * k} contiguous fp32 weights on y's device are needed")
     _need(out_dtype in _DT, f"out_dtype {out_dtype} is not supported")
     if y_shared is not None:
         _check(y_shared, "y_shared", (y.dtype,), (T, H))
@@ -430,6 +431,9 @@ def q4_matvec(x: torch.Tensor, w: Q4Matrix, up: Q4Matrix | None = None, limit: f
     unsorted rows).  up: gate and up products and their clamped SwiGLU.  Rows of y behind offsets[-1] stay as they
     were (undefined when `out` is not given)."""
     _check(x, "x", _FLOATS, (-1, w.K))
+    dev = x.get_device()
+    _need(w.codes.get_device() == dev and (up is None or up.codes.get_device() == dev),
+          "the matrices are on another device than x")
     R = x.shape[0]
     if row_map is not None:
         _check(row_map, "row_map", _I32, (-1,))
