@@ -235,12 +235,6 @@ __global__ void __launch_bounds__(KW * WM * 32, (NT == 1 ? 16 : 12) / (KW * WM))
 
     for (int64_t r0 = row0; r0 < row1; r0 += kTile) {
         const int nr = (int)min((int64_t)kTile, row1 - r0);
-        if (tid < 8 * NT) {
-            const int64_t r = tid < nr ? (a.row_map ? a.row_map[r0 + tid] : r0 + tid) : -1;
-            s_x[tid] = r >= 0 && r < a.x_rows ? r * K * es : -1;
-        }
-        __syncthreads();
-
         // W, scales and zero points of the warp's i-th chunk (chunk warp + i * kWarps of the row) into a stage
         auto fetch_w = [&](int i, int stage, int kv) {  // kv: elements left, a multiple of 32
             const uint32_t at = stage * stage_bytes;
@@ -255,6 +249,18 @@ __global__ void __launch_bounds__(KW * WM * 32, (NT == 1 ? 16 : 12) / (KW * WM))
             if (sg < St::kGroups && sg * GB * 32 < kv) cp16(s_dst + at, s_src + i * sz_step);
             if (has_z && zg < St::kGroups && zg * GB * 32 < kv) cp16(z_dst + at, z_src + i * sz_step);
         };
+        const int runs = (chunks - warp + kWarps - 1) / kWarps;  // chunks of this warp
+        const int left0 = K - warp * kChunk;                     // elements from its first chunk on
+        constexpr int kStep = kWarps * kChunk;
+#pragma unroll
+        for (int i = 0; i < S - 1; ++i)  // W does not wait for the row map
+            if (i < runs) fetch_w(i, i, left0 - i * kStep);
+        if (tid < 8 * NT) {
+            const int64_t r = tid < nr ? (a.row_map ? a.row_map[r0 + tid] : r0 + tid) : -1;
+            s_x[tid] = r >= 0 && r < a.x_rows ? r * K * es : -1;
+        }
+        __syncthreads();
+
         // x, at most two rows: lane l holds unit l % 16 of row l / 16
         uint4 held[F32 ? 2 : 1];
         const int64_t x_off = HELD && (lane >> 4) < nr ? s_x[lane >> 4] : -1;
@@ -333,15 +339,10 @@ __global__ void __launch_bounds__(KW * WM * 32, (NT == 1 ? 16 : 12) / (KW * WM))
 #pragma unroll
         for (int j = 0; j < NT; ++j) ok[j] = 8 * j + g < kTile && s_x[8 * j + g] >= 0;
 
-        const int runs = (chunks - warp + kWarps - 1) / kWarps;  // chunks of this warp
-        const int left0 = K - warp * kChunk;                     // elements from its first chunk on
-        constexpr int kStep = kWarps * kChunk;
 #pragma unroll
         for (int i = 0; i < S - 1; ++i) {
-            if (i < runs) {
-                fetch_w(i, i, left0 - i * kStep);
-                if constexpr (!HELD) fetch_x(i, i, left0 - i * kStep);
-            }
+            if constexpr (!HELD)
+                if (i < runs) fetch_x(i, i, left0 - i * kStep);
             cp_commit();
         }
         if constexpr (HELD) {
