@@ -197,6 +197,31 @@ def test_clamp_exl3_tcgen05_gemm(clamp_exl3):
     _clamp_case(clamp_exl3, 256, "exl3 tcgen05 T=256")
 
 
+@pytest.mark.parametrize("fmt,path,n", [("q8_0", "gemv", 12), ("q8_0", "simt", 12), ("q8_0", "tc", 140), ("q8_0", "tc1", 140),
+                                        ("q8_0_f32", "gemv", 12), ("exl3", "gemv", 12), ("exl3", "tc", 140)])
+def test_clamp_keeps_nans(fmt, path, n):
+    """A NaN in a row reaches that row's output on every expert path (moe_ref.py:81-84: np.minimum and np.clip pass a
+    NaN on), and no other row's."""
+    moe.init(0)
+    f32 = fmt == "q8_0_f32"
+    cfg = synth.config("c0", tokens=n, fmt=fmt.split("_f32")[0])
+    if not f32:
+        cfg.x_dtype = "bf16"
+    b = Built(cfg)
+    L = b.make_layer(torch.float32, path=path)
+    rows = b.x_dev[:n].contiguous()
+    slots = torch.tensor([[i % 3, 3 + i % 2] for i in range(n)], dtype=torch.int32, device="cuda")
+    w = torch.full((n, 2), 0.5, dtype=torch.float32, device="cuda")
+    clean = L.forward_routed(rows, slots, w, y_dtype=torch.float32).clone()
+    bad = rows.clone()
+    bad[5, 100] = float("nan")
+    y = L.forward_routed(bad, slots, w, y_dtype=torch.float32)
+    L.check_device_error()
+    assert bool(y[5].isnan().all())
+    keep = [i for i in range(n) if i != 5]
+    assert torch.equal(y[keep], clean[keep]) and bool(clean.isfinite().all())
+
+
 # ----------------------------------------------------------------------------- fp32 clause
 @pytest.mark.parametrize("T", [1, 16, 256])
 def test_fp32_layers_meet_the_fp32_tolerance(T):

@@ -186,6 +186,43 @@ def test_infinities_and_nans_stay_in_their_row(dtype):
         assert torch.equal(y[r], y2[r])
 
 
+@pytest.mark.parametrize("limit", [10.0, float("inf")])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N", [64, 9504])                  # one tile a warp, and four
+@pytest.mark.parametrize("n", [2, 9, 40])
+def test_gate_up_keeps_nans_and_infinities(n, N, dtype, limit):
+    """The clamps of the fused SwiGLU pass a NaN on (max and min that drop it would store numbers that look sound), as
+    its definition does; a row of +inf gives the clamped product, one of -inf silu(-inf) = -inf / inf = NaN."""
+    g = gen(11)
+    gate, up = (make((), N, 672, 32, torch.bfloat16, False, g) for _ in range(2))
+    for m in (gate, up):
+        m.codes |= 0x99                                    # q - 8 > 0 everywhere
+        m.scales.abs_()
+    blind = moe.Q4Matrix(torch.full_like(up.codes, 0x88), up.scales)   # q - 8 = 0: 0 for finite rows, NaN for infinite
+    x = torch.randn(n, 672, generator=g, device="cuda").to(dtype)
+    bad = {0: float("nan"), 1: float("inf")}
+    if n > 2:
+        bad[8] = float("-inf")
+    x2 = x.clone()
+    for r, v in bad.items():
+        x2[r, 77 * (r + 1) % 672] = v
+    clean, got = moe.q4_matvec(x, gate, up=up, limit=limit), moe.q4_matvec(x2, gate, up=up, limit=limit)
+    assert bool(got[0].isnan().all())
+    if limit == float("inf"):
+        assert bool((got[1] == limit).all())
+    else:                                                  # silu(10) * 10: the formula's error as in swiglu64, rounded once
+        want = torch.full((N,), limit * limit / (1.0 + np.exp(-limit)), dtype=torch.float64, device="cuda")
+        within(got[1], want, 8 * V * want, dtype)
+    if n > 2:
+        assert bool(got[8].isnan().all())
+    for r in range(n):
+        if r not in bad:
+            assert torch.equal(got[r], clean[r]) and bool(got[r].isfinite().all())
+    half = moe.q4_matvec(x2, gate, up=blind, limit=limit)  # a NaN of the up product alone
+    for r in range(n):
+        assert bool(half[r].isnan().all()) if r in bad else bool((half[r] == 0).all())
+
+
 def test_fp32_rows_keep_their_bits():
     """fp32 rows that differ from bf16 ones in their last bits: the product follows them."""
     g = gen(5)

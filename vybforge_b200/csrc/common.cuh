@@ -88,18 +88,30 @@ __device__ __forceinline__ void st_act(void *p, int64_t i, float v, int dtype) {
     else reinterpret_cast<float *>(p)[i] = v;
 }
 
+// min and max that pass a NaN on, as np.minimum and np.clip do; fminf and fmaxf return the other operand
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // Clamped SwiGLU of native/glm53/moe_ref.py:81-84: silu(min(g, L)) * clip(u, -L, L).
 __device__ __forceinline__ float swiglu_clamped(float g, float u, float lim) {
-    g = fminf(g, lim);
-    u = fminf(fmaxf(u, -lim), lim);
+    g = min_nan(g, lim);
+    u = min_nan(max_nan(u, -lim), lim);
     return (g / (1.0f + expf(-g))) * u;
 }
 
 // swiglu_clamped with the fast exponential and division intrinsics (a few ulp of fp32),
 // for epilogues whose result is rounded to fp16.
 __device__ __forceinline__ float swiglu_clamped_fast(float g, float u, float lim) {
-    g = fminf(g, lim);
-    u = fminf(fmaxf(u, -lim), lim);
+    g = min_nan(g, lim);
+    u = min_nan(max_nan(u, -lim), lim);
     return __fdividef(g, 1.0f + __expf(-g)) * u;
 }
 
