@@ -138,6 +138,28 @@ def test_combine_any_type_and_length(T, k, E, H, dtype, mode, shared):
         within(got, want, (k + 2) * V * size, out)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,k,H", [(1, 8, 6144), (32, 6, 6144), (260, 8, 1020), (260, 3, 1028), (130, 6, 2052), (300, 16, 1024),
+                                   (64, 9, 4096), (2050, 2, 132), (1040, 5, 264), (5, 2, 70000)])
+def test_words_of_every_width_give_the_same_bits(T, k, H, dtype):
+    """Row lengths and counts on both sides of each rule that chooses 16-byte words, 8-byte words, columns or the
+    layer's kernel: the values are those of the definition, and the bits those of the element path."""
+    _, pos, n, y, w, g = rows_case(T, k, 16, H, dtype, "dropped", seed=14)
+    v, kept = gathered(y, pos, T, k)
+    t = torch.where(kept, v * w.double().view(T, k, 1), 0.0)
+    ys = torch.randn(T, H, device="cuda", generator=g).to(dtype)
+    y1 = torch.empty(y.numel() + 1, dtype=dtype, device="cuda")[1:].view(y.shape).copy_(y)   # no word begins at its address
+    for shared in (None, ys):
+        want, size = t.sum(1), t.abs().sum(1)
+        if shared is not None:
+            want, size = want + ys.double(), size + ys.double().abs()
+        for out in DTYPES:
+            got = moe.combine(y, pos, w, T, k, y_shared=shared, out_dtype=out)
+            within(got, want, (k + 2) * V * size, out)
+            assert torch.equal(got, moe.combine(y1, pos, w, T, k, y_shared=shared, out_dtype=out))
+    assert torch.equal(moe.permute_backward(y, pos, T, k), moe.permute_backward(y1, pos, T, k))
+
+
 @pytest.mark.parametrize("mode", ["plain", "dropped", "none"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,k,E,H", SHAPES[:9])

@@ -565,22 +565,39 @@ int launch_permute(const int32_t *idx, int64_t T, int k, int E, const void *x, i
     return permute_launch<uint16_t>(idx, T, k, E, x, xs, H, counts, offsets, perm_tok, pos_of, st);
 }
 
-// 16-byte words of y (8 columns of a 16-bit type, 4 of fp32) where rows and addresses allow, else columns.
+// 16-byte words of y (8 columns of a 16-bit type, 4 of fp32) where rows and addresses allow, else 8-byte words of a 16-bit
+// type, else columns.  All forms add in the same order, so the bits are the same.  Few rows of a 16-bit type go in 8-byte words
+// too (twice the threads, half of each one's loads to wait for).  Many rows in words of four columns take the layer's
+// combine_kernel (32 registers a thread against 43, CTAs of 1,024 columns), where they fill its CTAs and k leaves at most three
+// lanes to its loop of eight, which takes a remainder one lane at a time.  B200, bf16 out with shared rows, us (inputs larger
+// than L2 at T = 4096):
+//   fp16, H = 6144, k = 8: T = 1 8-byte words 1.86, 16-byte 2.38;  T = 4096 94.1, 83.9
+//   fp16, H = 1020, T = 4096: k = 8 combine_kernel 18.1, 8-byte words 18.8, columns 40.8;  k = 6 20.5, 17.2, 52.9
+//   fp32, H = 6144, T = 4096: k = 2 combine_kernel 64.3, 16-byte words 77.2;  k = 8 141, 151;  k = 6 131, 130
+//   fp32, T = 32, H = 6144, k = 6: 2.82, 2.18;  T = 4096, H = 512, k = 6: 16.2, 12.6
 int launch_return_rows(const void *y, int y_dtype, const int32_t *pos_of, const float *w, int64_t T, int64_t H, int k,
                        const void *y_shared, void *out, int out_dtype, cudaStream_t st) {
-    const int ve = 16 / elem_size(y_dtype);
-    const int64_t oa = ve * elem_size(out_dtype) < 16 ? ve * elem_size(out_dtype) : 16;
-    const bool wide = H % ve == 0 && aligned(y, 16) && aligned(y_shared, 16) && aligned(out, oa);
+    const int es = elem_size(y_dtype), os = elem_size(out_dtype);
+    const bool many = T * H >= (int64_t)1 << 18;
+    // words of n columns: the rows' length and all addresses allow them
+    auto words = [&](int n) {
+        return H % n == 0 && aligned(y, n * es) && aligned(y_shared, n * es) && aligned(out, n * os < 16 ? n * os : 16);
+    };
+    const bool full = many && H > 512 && H <= 65535 * 1024 && k % 8 < 4;
 #define VF_RETURN(DT, VE) return return_launch<DT, VE>(y, pos_of, w, T, H, k, y_shared, out, out_dtype, st)
-    if (y_dtype == VFMOE_DT_F32) {
-        if (wide) VF_RETURN(VFMOE_DT_F32, 4);
-        VF_RETURN(VFMOE_DT_F32, 1);
+    if (y_dtype != VFMOE_DT_F32 && words(8) && many) {
+        if (y_dtype == VFMOE_DT_F16) VF_RETURN(VFMOE_DT_F16, 8);
+        VF_RETURN(VFMOE_DT_BF16, 8);
     }
-    if (y_dtype == VFMOE_DT_F16) {
-        if (wide) VF_RETURN(VFMOE_DT_F16, 8);
-        VF_RETURN(VFMOE_DT_F16, 1);
+    if (words(4)) {
+        if (full && y_dtype != VFMOE_DT_BF16)
+            return launch_combine(y, y_dtype, pos_of, w, (int)T, (int)H, k, y_shared, out, out_dtype, st);
+        if (y_dtype == VFMOE_DT_F32) VF_RETURN(VFMOE_DT_F32, 4);
+        if (y_dtype == VFMOE_DT_F16) VF_RETURN(VFMOE_DT_F16, 4);
+        VF_RETURN(VFMOE_DT_BF16, 4);
     }
-    if (wide) VF_RETURN(VFMOE_DT_BF16, 8);
+    if (y_dtype == VFMOE_DT_F32) VF_RETURN(VFMOE_DT_F32, 1);
+    if (y_dtype == VFMOE_DT_F16) VF_RETURN(VFMOE_DT_F16, 1);
     VF_RETURN(VFMOE_DT_BF16, 1);
 #undef VF_RETURN
 }
