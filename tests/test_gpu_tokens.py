@@ -160,6 +160,31 @@ def test_words_of_every_width_give_the_same_bits(T, k, H, dtype):
     assert torch.equal(moe.permute_backward(y, pos, T, k), moe.permute_backward(y1, pos, T, k))
 
 
+def test_combine_takes_longer_buffers_and_more_tokens():
+    """Buffers with room for more tokens than the call has (the positions, the weights and the shared rows), and more
+    lanes than a sorted plan may have: 2^27 + 1 tokens of 8 lanes, almost all without a row."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    T, k, H, room = 5, 2, 64, 9
+    y = torch.randn(room * k, H, device="cuda", generator=g)
+    pos = torch.randperm(room * k, device="cuda", generator=g).int()
+    w = torch.rand(room, k, device="cuda", generator=g)
+    ys = torch.randn(room, H, device="cuda", generator=g)
+    whole = moe.combine(y, pos, w, room, k, y_shared=ys, out_dtype=torch.float32)
+    assert torch.equal(moe.combine(y, pos, w, T, k, y_shared=ys, out_dtype=torch.float32), whole[:T])
+    assert torch.equal(moe.combine(y, pos, w, T, k, y_shared=ys.view(1, room, H), out_dtype=torch.float32), whole[:T])
+    with pytest.raises(_lib.VfmoeError):
+        moe.combine(y, pos, w, T, k, y_shared=ys[:T - 1])
+    T, k, H = (1 << 27) + 1, 8, 4
+    y = torch.randn(16, H, device="cuda", generator=g).half()
+    pos = torch.full((T * k,), -1, dtype=torch.int32, device="cuda")
+    pos[:8] = torch.arange(8, dtype=torch.int32, device="cuda")
+    pos[-8:] = torch.arange(8, 16, dtype=torch.int32, device="cuda")
+    out = moe.combine(y, pos, None, T, k, out_dtype=torch.float16)
+    v = y.double().view(2, 8, H)
+    within(out[[0, T - 1]], v.sum(1), (k + 2) * V * v.abs().sum(1), torch.float16)
+    assert int(out.count_nonzero()) <= 2 * H
+
+
 @pytest.mark.parametrize("mode", ["plain", "dropped", "none"])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,k,E,H", SHAPES[:9])

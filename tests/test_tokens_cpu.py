@@ -45,3 +45,10 @@ def test_nothing_to_do_is_no_error(built_lib):
     assert built_lib.vfmoe_combine(0, 0, 0, 0, 0, 2, 64, 0, 0, 0, 0) == _lib.OK
     assert built_lib.vfmoe_combine_backward(0, 0, 0, 0, 0, 0, 0, 2, 64, 0, 0, 0) == _lib.OK
     assert built_lib.vfmoe_permute_backward(0, 0, 0, 0, 2, 64, 0, 0, 0) == _lib.OK
+
+
+@pytest.mark.parametrize("kw", [dict(T=1 << 31), dict(H=1 << 31), dict(k=33), dict(T=1 << 27, k=64)])
+def test_combine_refuses_what_passes_its_indices(built_lib, kw):
+    a = dict(T=4, k=2, H=64)
+    a.update(kw)
+    assert built_lib.vfmoe_combine(A, 0, A, 0, a["T"], a["k"], a["H"], 0, A, 0, 0) == _lib.ERR_INVALID

@@ -731,9 +731,10 @@ static bool lanes_ok(int64_t T, int64_t k, int64_t H) {
 
 int vfmoe_combine(int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w, int64_t T, int64_t k, int64_t H,
                   int64_t y_shared, int64_t out, int64_t out_dtype, int64_t stream) {
-    if (!lanes_ok(T, k, H) || !is_float_dtype(y_dtype) || !is_float_dtype(out_dtype) ||
-        (T > 0 && (!y || !pos_of || !out)) || (y | y_shared) % dtype_bytes(y_dtype) || out % dtype_bytes(out_dtype) ||
-        (pos_of | w) % 4) {
+    // no plan bounds the tokens: expert-parallel buffers may hold more lanes than vfmoe_permute sorts
+    if (T < 0 || T > INT32_MAX || k <= 0 || k > 32 || H <= 0 || H > INT32_MAX || !is_float_dtype(y_dtype) ||
+        !is_float_dtype(out_dtype) || (T > 0 && (!y || !pos_of || !out)) || (y | y_shared) % dtype_bytes(y_dtype) ||
+        out % dtype_bytes(out_dtype) || (pos_of | w) % 4) {
         set_error("vfmoe_combine: bad arguments");
         return VFMOE_ERR_INVALID;
     }

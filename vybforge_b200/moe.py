@@ -341,7 +341,8 @@ def permute_backward(dxs: torch.Tensor, pos_of: torch.Tensor, T: int, k: int, ou
 
 def combine(y: torch.Tensor, pos_of: torch.Tensor, w, T: int, k: int, y_shared=None,
             out_dtype=torch.bfloat16) -> torch.Tensor:
-    """out[t] = sum_l w[t,l] * y[pos_of[t*k+l]] (+ y_shared[t]); y fp32, fp16 or bf16; pos < 0 skips."""
+    """out[t] = sum_l w[t,l] * y[pos_of[t*k+l]] (+ y_shared[t]); y fp32, fp16 or bf16; pos < 0 skips.  pos_of, w and
+    y_shared may hold more tokens than T."""
     _check(y, "y", _FLOATS, (-1, -1))
     H = y.shape[1]
     dev = y.get_device()
@@ -351,7 +352,8 @@ def combine(y: torch.Tensor, pos_of: torch.Tensor, w, T: int, k: int, y_shared=N
                         w.get_device() == dev), f"w: {T * k} contiguous fp32 weights on y's device are needed")
     _need(out_dtype in _DT, f"out_dtype {out_dtype} is not supported")
     if y_shared is not None:
-        _check(y_shared, "y_shared", (y.dtype,), (T, H))
+        _need(y_shared.dtype == y.dtype and y_shared.is_contiguous() and y_shared.numel() >= T * H and
+              y_shared.get_device() == dev, f"y_shared: {T} contiguous rows of {H} of y's dtype on y's device are needed")
     out = y.new_empty((T, H), dtype=out_dtype)
     check(_lib.load().vfmoe_combine(_ptr(y), _DT[y.dtype], _ptr(pos_of), _ptr(w), T, k, H, _ptr(y_shared), _ptr(out),
                                     _DT[out_dtype], _stream()))
