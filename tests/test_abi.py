@@ -145,3 +145,29 @@ def test_pack_load_rejects_a_file_that_is_not_a_pack(built_lib, tmp_path):
     assert built_lib.vfmoe_pack_bytes(str(p).encode()) == _lib.ERR_INVALID
     assert "not a version-1 vfmoe pack" in _lib.last_error()
     assert built_lib.vfmoe_pack_bytes(str(tmp_path / "missing").encode()) == _lib.ERR_INVALID
+
+
+def test_stream_handle_without_torchs_undocumented_call(monkeypatch):
+    """A torch that lacks the quick way to the current stream's handle: the documented one gives it."""
+    import importlib.util
+    import types
+
+    import torch
+
+    from vybforge_b200 import moe
+    monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: types.SimpleNamespace(cuda_stream=77))
+    spec = importlib.util.spec_from_file_location("vybforge_b200.moe_of_another_torch", moe.__file__)
+    other = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(other)
+    assert other._stream() == 77
+
+
+@pytest.mark.gpu
+def test_stream_handle_is_the_current_streams():
+    import torch
+
+    from vybforge_b200 import moe
+    assert moe._stream() == torch.cuda.current_stream().cuda_stream
+    with torch.cuda.stream(torch.cuda.Stream()) as _:
+        assert moe._stream() == torch.cuda.current_stream().cuda_stream != 0
