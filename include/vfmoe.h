@@ -505,7 +505,8 @@ int vfmoe_q4_matvec(const vfmoe_q4_matrix *w, const vfmoe_q4_matrix *up, double 
                     int64_t stream);
 
 /* [n_mats][n][k] values (F32, F16 or BF16, finite) -> dst's buffers, round to nearest.  Without zeros s =
- * max|w| / 7; with zeros the range of the group and 0 in 15 steps.  The scale is rounded to scale_dtype first. */
+ * max|w| / 7; with zeros the range of the group and 0 in 15 steps.  The scale is rounded to scale_dtype first; one
+ * past fp16's largest value takes that value, and elements out of its reach the end of the code range. */
 int vfmoe_q4_quantize(int64_t src, int64_t src_dtype, const vfmoe_q4_matrix *dst, int64_t stream);
 
 /* 4-bit matrices -> dense [n_mats][n][k] (F32, F16 or BF16): the fp32 product s * (q - z), rounded once. */

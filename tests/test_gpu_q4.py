@@ -260,6 +260,32 @@ def test_quantize_and_dequantize(G, zeros):
                 assert int(m.zeros.max()) <= 15
 
 
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("sd", [torch.float16, torch.bfloat16])
+def test_quantize_the_largest_finite_weights(sd, zeros):
+    """Finite weights give finite codes and scales: a scale past fp16's range takes its largest value and the far elements
+    the end of the code range, and a range that passes fp32 itself is no infinite scale."""
+    G, N, K = 64, 32, 256
+    g = gen(12)
+    w = torch.randn(N, K, generator=g, device="cuda")
+    w[:16] *= 1e6                                          # scales of about 2e5 to 4e5 where fp16 ends at 65,504
+    w[16:] = torch.where(w[16:] < 0, -2.5e38, 2.5e38) * torch.rand(16, K, generator=g, device="cuda")
+    w[:, ::G], w[:, 1::G] = w[:, ::G].abs(), -w[:, 1::G].abs()   # both signs in every group
+    m = moe.q4_quantize(w, group=G, scale_dtype=sd, zeros=zeros)
+    d = moe.q4_dequant(m)
+    assert bool(m.scales.isfinite().all()) and bool(d.isfinite().all())
+    s = m.scales.double().transpose(-1, -2).repeat_interleave(G, -1)
+    z = 8.0 if m.zeros is None else m.zeros.double().transpose(-1, -2).repeat_interleave(G, -1)
+    reach = (w.double().clamp(-z * s, (15.0 - z) * s) - d.double()).abs()      # half a step, and the quotient's rounding
+    assert bool((reach <= s * (0.5 + 16 * V)).all())
+    if sd == torch.float16:
+        assert bool((m.scales == 65504).all())
+    else:                                                  # as in test_quantize_and_dequantize
+        u, top = torch.finfo(sd).eps / 2, 15.0 if zeros else 7.0
+        step = s * ((1.0 if zeros else 0.5) + 2 * top * u + 16 * V)
+        assert bool(((d - w).double().abs() <= step).all())
+
+
 def test_no_rows_and_one_stream():
     g = gen(6)
     m = make((), 32, 64, 32, torch.bfloat16, False, g)

@@ -29,8 +29,13 @@ __global__ void __launch_bounds__(128) q4_quantize_kernel(const void *__restrict
         lo = fminf(lo, v);
         hi = fmaxf(hi, v);
     }
-    const float want = zeros ? __fdiv_rn(__fsub_rn(hi, lo), 15.f) : __fdiv_rn(fmaxf(hi, -lo), 7.f);
-    const uint16_t bits = scale_bits(want, scale_f16);
+    float want = __fdiv_rn(fmaxf(hi, -lo), 7.f);
+    if (zeros) {
+        const float range = __fsub_rn(hi, lo);  // of finite values, yet it may pass fp32
+        want = isinf(range) ? __fsub_rn(__fdiv_rn(hi, 15.f), __fdiv_rn(lo, 15.f)) : __fdiv_rn(range, 15.f);
+    }
+    uint16_t bits = scale_bits(want, scale_f16);
+    if (scale_f16 && bits == 0x7c00) bits = 0x7bff;  // past fp16: its largest value, an infinite scale would make zeros NaN
     const float s = q4_scale(bits, scale_f16);
     float z = 8.f;
     if (zeros) z = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(-lo, s)), 0.f), 15.f) : 0.f;
