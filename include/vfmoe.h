@@ -214,8 +214,9 @@ int vfmoe_forward_rows(int64_t handle, int64_t rows, int64_t rows_dtype, int64_t
 /* Weighted combine: out[t] = sum_l w[t,l] * y[pos_of[t*k+l]] + y_shared[t].  y rows and
  * y_shared are y_dtype F32, F16 or BF16; w may be 0 for weight 1; y_shared may
  * be 0; a negative pos_of entry skips that lane (its weight is not read into the sum).  out_dtype
- * F32, BF16 or F16.  Any H; H a multiple of 16 bytes of y and 16-byte aligned pointers move 16-byte
- * words.  Lanes are added in lane order in fp32, one rounding.  glm_engine.vyb:2925-2938, :2991. */
+ * F32, BF16 or F16.  Any H; H a multiple of 4 and aligned pointers move words of 8 or 16 bytes.  Lanes
+ * are added in lane order in fp32, one rounding.  out must not overlap y or y_shared.
+ * glm_engine.vyb:2925-2938, :2991. */
 int vfmoe_combine(int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w, int64_t T, int64_t k, int64_t H,
                   int64_t y_shared, int64_t out, int64_t out_dtype, int64_t stream);
 
@@ -223,8 +224,8 @@ int vfmoe_combine(int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w, int64_t
  * (dout_dtype): for every lane with pos = pos_of[t*k+l] >= 0
  *   dy[pos] = w[t,l] * dout[t]        (y_dtype, one rounding; rows that no lane names stay as they were)
  *   dw[t,l] = <dout[t], y[pos]>       (fp32; 0 for a lane without a row)
- * dy or dw may be 0 (y is read for dw only); w = 0: weight 1; dy may be y itself.  The gradient of
- * y_shared is dout.  The positions are those of a plan: no two lanes name one row.  No counterpart in the
+ * dy or dw may be 0 (y is read for dw only); w = 0: weight 1; dy may be y itself, but overlap neither a part
+ * of y nor dout.  The gradient of y_shared is dout.  The positions are those of a plan: no two lanes name one row.  No counterpart in the
  * reference, whose MoE path is forward only. */
 int vfmoe_combine_backward(int64_t dout, int64_t dout_dtype, int64_t y, int64_t y_dtype, int64_t pos_of, int64_t w,
                            int64_t T, int64_t k, int64_t H, int64_t dy, int64_t dw, int64_t stream);

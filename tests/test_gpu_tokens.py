@@ -378,3 +378,33 @@ def test_refusals():
             call()
         assert e.value.code == _lib.ERR_INVALID, i
     torch.cuda.synchronize()
+
+
+def test_outputs_that_overlap_inputs_are_refused():
+    """One lane a token and square matrices make shapes that fit in place: the kernels would read rows others wrote."""
+    T, H = 16, 64
+    idx = torch.zeros((T, 1), dtype=torch.int32, device="cuda")
+    buf = torch.zeros(T * H + 64, device="cuda")
+    x, near = buf[:T * H].view(T, H), buf[64:].view(T, H)
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    y = torch.zeros((T, H), device="cuda")
+    m = moe.q4_quantize(torch.randn(H, H, device="cuda"), group=32)
+    bad = [
+        lambda: moe.permute(x, idx, 4, out=x),
+        lambda: moe.permute(x, idx, 4, out=near),
+        lambda: moe.permute(near, idx, 4, out=x),
+        lambda: moe.combine_backward(x, y, pos, None, T, 1, dy=x),
+        lambda: moe.combine_backward(y, x, pos, None, T, 1, dy=near),
+        lambda: moe.q4_matvec(x, m, out=x),
+        lambda: moe.q4_matvec(near, m, out=x),
+    ]
+    for i, call in enumerate(bad):
+        with pytest.raises(_lib.VfmoeError, match="overlaps") as e:
+            call()
+        assert e.value.code == _lib.ERR_INVALID, i
+    dy, _ = moe.combine_backward(y, x, pos, None, T, 1, dy=x)                 # the rows themselves are allowed
+    assert dy.data_ptr() == x.data_ptr()
+    halves = torch.zeros((2 * T, H), device="cuda")                            # neighbours in one buffer are apart
+    moe.permute(halves[:T], idx, 4, out=halves[T:])
+    moe.q4_matvec(halves[T:], m, out=halves[:T])
+    torch.cuda.synchronize()

@@ -295,6 +295,13 @@ def _check(t: torch.Tensor, name: str, dtypes, shape) -> None:
                                       f"{'' if t.is_contiguous() else ', not contiguous'}")
 
 
+def _check_apart(out: torch.Tensor, name: str, t: torch.Tensor, other: str) -> None:
+    """The kernels write out while others of their CTAs read t: the two must not share memory."""
+    a, b = out.data_ptr(), t.data_ptr()
+    if a < b + t.nbytes and b < a + out.nbytes:
+        raise VfmoeError(ERR_INVALID, f"{name} overlaps {other}")
+
+
 _I32, _F32, _FLOATS = (torch.int32,), (torch.float32,), (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -310,7 +317,7 @@ class Plan(NamedTuple):
 def permute(x: torch.Tensor | None, idx: torch.Tensor, n_experts: int, out: torch.Tensor | None = None):
     """(xs, Plan): the rows of x [T, H] sorted by the expert ids idx int32 [T, k], xs [T*k, H] of x's dtype
     (vfmoe_permute).  An id outside [0, n_experts) drops its lane; the rows of xs behind offsets[-1] stay as
-    they were (undefined when `out` is not given).  x=None makes the plan alone (xs None)."""
+    they were (undefined when `out` is not given).  `out` must not overlap x.  x=None makes the plan alone (xs None)."""
     _check(idx, "idx", _I32, (-1, -1))
     T, k = idx.shape
     H, dt, xs = 0, DT_F32, None
@@ -321,6 +328,7 @@ def permute(x: torch.Tensor | None, idx: torch.Tensor, n_experts: int, out: torc
             xs = x.new_empty((T * k, H))
         else:
             _check(out, "out", (x.dtype,), (T * k, H))
+            _check_apart(out, "out", x, "x")
             xs = out
     _need(0 < n_experts <= 1024, f"n_experts = {n_experts}: 1 to 1024 are supported")
     n = T * k  # one allocation for the plan
@@ -369,7 +377,8 @@ def combine(y: torch.Tensor, pos_of: torch.Tensor, w, T: int, k: int, y_shared=N
 def combine_backward(dout: torch.Tensor, y: torch.Tensor, pos_of: torch.Tensor, w: torch.Tensor | None, T: int, k: int,
                      dy: torch.Tensor | None = None):
     """(dy, dw fp32 [T, k]) of combine from dout [T, H] (vfmoe_combine_backward).  dy has y's shape and dtype
-    and may be y itself; its rows that no lane names stay as they were (undefined when `dy` is not given).
+    and may be y itself, but overlap neither a part of y nor dout; its rows that no lane names stay as they were (undefined
+    when `dy` is not given).
     The gradient of combine's y_shared is dout."""
     _check(y, "y", _FLOATS, (-1, -1))
     H = y.shape[1]
@@ -381,6 +390,9 @@ def combine_backward(dout: torch.Tensor, y: torch.Tensor, pos_of: torch.Tensor, 
         dy = torch.empty_like(y)
     else:
         _check(dy, "dy", (y.dtype,), y.shape)
+        _check_apart(dy, "dy", dout, "dout")
+        if dy.data_ptr() != y.data_ptr():
+            _check_apart(dy, "dy", y, "y, but is not y")
     dw = y.new_empty((T, k), dtype=torch.float32)
     check(_lib.load().vfmoe_combine_backward(_ptr(dout), _DT[dout.dtype], _ptr(y), _DT[y.dtype], _ptr(pos_of), _ptr(w),
                                              T, k, H, _ptr(dy), _ptr(dw), _stream()))
@@ -434,10 +446,10 @@ def q4_dequant(w: Q4Matrix, dtype=torch.float32) -> torch.Tensor:
 def q4_matvec(x: torch.Tensor, w: Q4Matrix, up: Q4Matrix | None = None, limit: float = 10.0,
               offsets: torch.Tensor | None = None, row_map: torch.Tensor | None = None,
               out: torch.Tensor | None = None, out_dtype=None) -> torch.Tensor:
-    """y [R, N] = the rows of x [.., K] times w^T (vfmoe_q4_matvec).  offsets int32 [E + 1]: the rows are sorted
+    """y [R, N] = the rows of x [M, K] times w^T (vfmoe_q4_matvec).  offsets int32 [E + 1]: the rows are sorted
     by matrix (permute's plan); row_map int32 [R]: the row of x of each row of y (the plan's perm_tok reads the
     unsorted rows).  up: gate and up products and their clamped SwiGLU.  Rows of y behind offsets[-1] stay as they
-    were (undefined when `out` is not given)."""
+    were (undefined when `out` is not given).  `out` must not overlap x."""
     _check(x, "x", _FLOATS, (-1, w.K))
     dev = x.get_device()
     _need(w.codes.get_device() == dev and (up is None or up.codes.get_device() == dev),
@@ -454,6 +466,7 @@ def q4_matvec(x: torch.Tensor, w: Q4Matrix, up: Q4Matrix | None = None, limit: f
         out = x.new_empty((R, w.N), dtype=out_dtype)
     else:
         _check(out, "out", _FLOATS if out_dtype is None else (out_dtype,), (R, w.N))
+        _check_apart(out, "out", x, "x")
     check(_lib.load().vfmoe_q4_matvec(C.byref(w.desc), None if up is None else C.byref(up.desc), limit, _ptr(x),
                                       _DT[x.dtype], x.shape[0], _ptr(row_map), _ptr(offsets), R, _ptr(out),
                                       _DT[out.dtype], _stream()))
