@@ -500,7 +500,10 @@ typedef struct vfmoe_q4_matrix {
  * entry outside [0, x_rows) reads as a row of zeros.  y must not overlap x.
  * up != 0: a second matrix of the same kind, y = silu(min(W x, limit)) * clip(up x, -limit, limit)
  * (moe_ref.py:81-84; limit > 0, infinity for none).  q - z is exact in the tensor cores' operands, and so is x (fp32
- * x as three bf16 parts): sums, the group scales and the SwiGLU are fp32, one rounding to y_dtype. */
+ * x as three bf16 parts): sums, the group scales and the SwiGLU are fp32, one rounding to y_dtype.  A group's sum of
+ * (q - z) x is formed before its scale, so a row keeps |x| below 3.4e38 / (15 group), 1.7e35 at group 128: beyond, the
+ * sum may pass fp32 where the scaled one would not.  A NaN, and an infinity that meets q = z, make the row's outputs NaN,
+ * through the SwiGLU too. */
 int vfmoe_q4_matvec(const vfmoe_q4_matrix *w, const vfmoe_q4_matrix *up, double limit, int64_t x, int64_t x_dtype,
                     int64_t x_rows, int64_t row_map, int64_t offsets, int64_t rows, int64_t y, int64_t y_dtype,
                     int64_t stream);

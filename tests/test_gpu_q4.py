@@ -144,6 +144,76 @@ def test_experts(E, T, k, N, K, G, mode):
         assert bool((h[n:] == 3.0).all())
 
 
+# A dense call's layout goes by the channels (N = 208: warps along K, 8 of them; 4,752: one tile of channels, 4 warps along K;
+# 9,488: two tiles, or with gate and up four; 18,960: four; a few more than 64, 128 and 512 in each) and by the rows (1: held in
+# registers; 5: one tile of 8; 13: 16 rows, along K or from 9,472 channels on with x shared by warps; 45: 32 and 13 rows, the
+# same), each for every type of x, group, type of scale, and with or without gate and up: these are all kernels there are.
+# K is 19 chunks of 128 and a part of one, so every ring turns and ends inside a chunk.
+@pytest.mark.parametrize("sdtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("G", [32, 64, 128])
+@pytest.mark.parametrize("N", [208, 4752, 9488, 18960])
+def test_every_layout_of_a_dense_product(N, G, sdtype):
+    K = 19 * 128 + {32: 96, 64: 64, 128: 0}[G]
+    g = gen(N + G)
+    for zeros in (False, True):
+        gate, up = make((), N, K, G, sdtype, zeros, g), make((), N, K, G, sdtype, zeros, g)
+        wg, wu = dense64(gate), dense64(up)
+        for dtype in DTYPES:
+            for n in (1, 5, 13, 45):
+                x = torch.randn(n, K, generator=g, device="cuda").to(dtype)
+                a, ea = product64(wg, x.double(), dtype)
+                b, eb = product64(wu, x.double(), dtype)
+                within(moe.q4_matvec(x, gate), a, ea, dtype)
+                want, err = swiglu64(a, ea, b, eb, 2.0)
+                within(moe.q4_matvec(x, gate, up=up, limit=2.0), want, err, dtype)
+
+
+# The same for sorted rows, whose layout goes by the rows a matrix has on average: held, 8, 16 along K, 16 and 32 with shared x,
+# 32 along K; and matrices with many times that ("one": all rows to one matrix, its tiles one after the other).
+@pytest.mark.parametrize("mode", ["plain", "dropped", "one"])
+@pytest.mark.parametrize("E,T,k,N,G", [(64, 2, 8, 624, 32), (64, 2, 8, 1200, 64), (64, 2, 8, 1200, 128), (16, 8, 4, 624, 128),
+                                       (16, 8, 4, 1200, 32), (16, 8, 4, 1200, 64), (16, 24, 4, 80, 64), (16, 24, 4, 624, 32),
+                                       (16, 24, 4, 640, 128), (16, 48, 4, 624, 64), (16, 48, 4, 1200, 32), (16, 48, 4, 1200, 128)])
+def test_every_layout_of_sorted_rows(E, T, k, N, G, mode):
+    K = 10 * 128 + {32: 96, 64: 64, 128: 0}[G]
+    for i, dtype in enumerate(DTYPES):
+        g = gen(E + T + N + i)
+        zeros, sd = (G // 32 + i) % 2 == 0, (torch.bfloat16, torch.float16)[i % 2]
+        gate, up = make((E,), N, K, G, sd, zeros, g), make((E,), N, K, G, sd, zeros, g)
+        x = torch.randn(T, K, generator=g, device="cuda").to(dtype)
+        _, plan = moe.permute(None, expert_rows(E, T, k, mode, g), E)
+        off = plan.offsets.tolist()
+        n = off[-1]
+        y = moe.q4_matvec(x, gate, offsets=plan.offsets, row_map=plan.perm_tok, out=torch.full((T * k, N), 3.0, dtype=dtype,
+                                                                                               device="cuda"))
+        h = moe.q4_matvec(x, gate, up=up, limit=0.5, offsets=plan.offsets, row_map=plan.perm_tok)
+        for e in range(E):
+            r = slice(off[e], off[e + 1])
+            if off[e] == off[e + 1]:
+                continue
+            rows = x[plan.perm_tok[r].long()].double()
+            m = [moe.Q4Matrix(w.codes[e], w.scales[e], None if w.zeros is None else w.zeros[e]) for w in (gate, up)]
+            a, ea = product64(dense64(m[0]), rows, dtype)
+            b, eb = product64(dense64(m[1]), rows, dtype)
+            within(y[r], a, ea, dtype)
+            want, err = swiglu64(a, ea, b, eb, 0.5)
+            within(h[r], want, err, dtype)
+        assert bool((y[n:] == 3.0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("G", [32, 64, 128])
+def test_rows_near_the_end_of_the_range(G, dtype):
+    """Group sums are formed before the scale: they hold while 15 G max|x| stays within fp32, as documented."""
+    g = gen(13)
+    m = make((), 48, 512, G, torch.bfloat16, True, g)
+    m.scales.copy_(2.0 ** -torch.randint(9, 12, m.scales.shape, generator=g, device="cuda"))
+    x = (torch.rand(5, 512, generator=g, device="cuda") * 2 - 1) * (3.3e38 / (15 * G))
+    x = x.to(dtype)
+    want, err = product64(dense64(m), x.double(), dtype)
+    within(moe.q4_matvec(x, m), want, err, dtype)
+
+
 @pytest.mark.parametrize("n", [1, 12, 40])
 def test_dense_gate_up(n):
     g = gen(n)

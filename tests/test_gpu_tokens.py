@@ -83,6 +83,30 @@ def test_permute_is_the_stable_order(T, k, E, H, mode):
     assert none is None and all(torch.equal(a, b) for a, b in zip(plan, again))
 
 
+@pytest.mark.parametrize("E", [1, 5, 256, 1024])
+@pytest.mark.parametrize("T,k,skew", [(8193, 8, 0.0), (8192, 8, 1.1), (32769, 8, 1.1), (131072, 2, 0.0), (70001, 1, 1.1)])
+def test_plans_of_many_lanes(T, k, skew, E):
+    """Above 65,536 lanes a warp's run of ids no longer fits its registers and is read in several passes; ids skewed towards a
+    few experts, repeated within a token, dropped on both sides of the range."""
+    rng = np.random.default_rng(T + E)
+    p = np.arange(1, E + 1) ** -skew
+    idx = rng.choice(rng.permutation(E), size=(T, k), p=p / p.sum()).astype(np.int32)
+    m = rng.random((T, k))
+    idx[m < 0.1] = -1
+    idx[m > 0.95] = E + 1
+    perm, pos, off = order(idx, E)
+    none, plan = moe.permute(None, torch.from_numpy(idx).cuda(), E)
+    x = torch.randn(T, 8, device="cuda").half()
+    xs, again = moe.permute(x, torch.from_numpy(idx).cuda(), E)
+    for got in (plan, again):
+        np.testing.assert_array_equal(got.pos_of.cpu().numpy(), pos)
+        np.testing.assert_array_equal(got.perm_tok.cpu().numpy(), perm)
+        np.testing.assert_array_equal(got.offsets.cpu().numpy(), off)
+        np.testing.assert_array_equal(got.counts.cpu().numpy(), np.diff(off))
+    n = int(off[-1])
+    assert torch.equal(xs[:n], x[torch.from_numpy(perm[:n]).cuda()])
+
+
 @pytest.mark.parametrize("T,k,E", [(37, 4, 16), (700, 8, 64)])
 def test_permute_plan_is_that_of_dispatch(T, k, E):
     idx = torch.from_numpy(make_ids(T, k, E, "plain", seed=3)).cuda()
