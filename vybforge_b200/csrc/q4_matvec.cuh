@@ -62,6 +62,8 @@ struct Zero {
         : c((F16 ? 0x64006400u : 0x43004300u) + z * 0x00010001u), d(0xd400d400u + z * 0x00100010u) {}
 };
 
+// Codes become operands by the known method of Kim, Henry, Fahim and Awadalla ("Who Says Elephants Can't Run", 2022): put into
+// the low bits of a float whose step there is one, then subtract.
 // The operand pairs (i, i + 4) of a word's codes less the zero point: base + q is exact with the code in the low bits of
 // base (bf16 128, fp16 1024), and so is its difference from base + z.  fp16 has room for the code four bits up: 1024 + 16 q,
 // and (1024 + 16 q) / 16 - (64 + z) is one exact fma, which saves two of the three shifts.  Shifts and masks run on the
@@ -560,6 +562,9 @@ int launch_few(const Q4Args &a, int64_t tiles, cudaStream_t st) {
 //   n = 16, N = 2048, K = 6144: along K 9.6 us (fp16), 64 CTAs of 32 channels 18.9
 //   n = 32, N = 131072, K = 6144: shared 265 us, along K 430;  n = 256, N = 6144: shared 115 us, along K 204
 //   n = 32, N = 2048, K = 6144: along K 20 us, shared 66;  n = 64, N = 6144, K = 2048: along K 24.5, shared 29
+// fp32 rows of more than 16 a tile always share x.  Along K they fit too (150 KB of shared memory), with a border of their own:
+//   n = 32, N = 2048, K = 6144: along K 48 us, shared 131;  N = 6144: 133, 139;  n = 24, N = 12288, K = 2048: 63, 47;
+//   n = 64, N = 6144, K = 2048: 95, 47
 template <int XD, int GB, bool ACT, bool SF16>
 int launch_rows(const Q4Args &a, cudaStream_t st) {
     constexpr int A = ACT ? 2 : 1;
@@ -575,7 +580,7 @@ int launch_rows(const Q4Args &a, cudaStream_t st) {
         return launch_tile<XD, 2, 2, GB, ACT, SF16, false, 1, 4, 3>(a, st);
     }
     const int64_t all = tiles * (a.offsets ? 1 : cdiv(a.rows, 32));
-    if constexpr (!F32)  // fp32 rows along K would not fit
+    if constexpr (!F32)
         if (all < 6 * A * kSms) return launch_tile<XD, 4, A, GB, ACT, SF16, false, 4, 1, 2>(a, st);
     return launch_tile<XD, 4, 2, GB, ACT, SF16, false, 1, 4, 3>(a, st);
 }
