@@ -61,3 +61,17 @@ def test_null_and_empty(built_lib):
     assert built_lib.vfmoe_q4_quantize(0, 0, C.byref(mat()), 0) == _lib.ERR_INVALID
     assert built_lib.vfmoe_q4_quantize(A, 4, C.byref(mat()), 0) == _lib.ERR_INVALID
     assert built_lib.vfmoe_q4_dequant(C.byref(mat()), A + 2, 0, 0) == _lib.ERR_INVALID
+
+
+def test_dequant_checks_where_the_matrix_lies():
+    """A matrix that is not on the current device is refused before its addresses reach a kernel of that device."""
+    import torch
+
+    from vybforge_b200 import moe
+    m = object.__new__(moe.Q4Matrix)                       # as if made while another device was current
+    m.codes, m.scales, m.zeros = torch.zeros(32, 64, dtype=torch.uint8), torch.zeros(4, 32).half(), None
+    m.N, m.K, m.group, m.n_mats = 32, 128, 32, 1
+    m.desc = mat(zeros=0, scale_dtype=_lib.DT_F16)
+    with pytest.raises(_lib.VfmoeError) as e:
+        moe.q4_dequant(m)
+    assert e.value.code == _lib.ERR_INVALID and "current" in str(e.value)

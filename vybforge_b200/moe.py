@@ -438,6 +438,7 @@ def q4_quantize(w: torch.Tensor, group: int = 128, scale_dtype=torch.bfloat16, z
 def q4_dequant(w: Q4Matrix, dtype=torch.float32) -> torch.Tensor:
     """Dense [N, K] or [E, N, K] of 4-bit matrices (vfmoe_q4_dequant)."""
     _need(dtype in _DT, f"dtype {dtype} is not supported")
+    _check(w.codes, "the matrix's codes", (torch.uint8,), w.codes.shape)
     out = w.codes.new_empty(tuple(w.codes.shape[:-1]) + (w.K,), dtype=dtype)
     check(_lib.load().vfmoe_q4_dequant(C.byref(w.desc), _ptr(out), _DT[dtype], _stream()))
     return out
